@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cstdlib>
 
+#include "launch.cuh"
 #include "chunk_kernels.cuh"
 #include "tc_bwd.cuh"
 #include "tc_scan.cuh"
@@ -279,12 +280,7 @@ Params make_params(const AtlasMemShape* s, const Layout& L, const AtlasMemFwd* f
   return P;
 }
 
-// ---- launch accounting and optional per-kernel CUDA-event timing ----------
-enum KernelId {
-  KID_FMAP_FWD, KID_FWD_CHUNK, KID_FWD_SCAN, KID_FWD_OUT, KID_BUF_OUT, KID_BWD_CHUNK, KID_BWD_SCAN,
-  KID_BWD_GRADS, KID_BWD_BUFOUT, KID_BWD_FINAL, KID_BWD_DSREF, KID_FMAP_BWD, KID_FWD_CHUNK_TC, KID_FWD_OUT_TC, KID_FWD_BUF_Y,
-  KID_BWD_CHUNK_TC, KID_BWD_STATE_GATES_TC, KID_BWD_BUF_TC, KID_BWD_FINAL_TC, KID_BWD_DSREF_TC, KID_BWD_KEYS_TC, KID_SREF_TILE, KID_DECODE, KID_SCAN_OP_FWD, KID_SCAN_OP_BWD, KID_CARRY, KID_DWCONV_FWD, KID_DWCONV_BWD, KID_HEADPREP_FWD, KID_HEADPREP_BWD, KID_PROJ_TILES, KID_FMAP_FWD_TC, KID_FMAP_BWD_TC, KID_OMEGA_STORE_FWD, KID_OMEGA_STORE_BWD, KID_AFFINE_FWD, KID_AFFINE_BWD, KID_COUNT
-};
+// ---- launch accounting and optional per-kernel CUDA-event timing (launch.cuh) ----------
 const char* const kKernelNames[KID_COUNT] = {
   "k_fmap_tensor_fwd", "k_fwd_chunk", "k_fwd_scan", "k_fwd_out", "k_buf_out", "k_bwd_chunk", "k_bwd_scan",
   "k_bwd_grads", "k_bwd_bufout", "k_bwd_finalize", "k_bwd_dsref", "k_fmap_tensor_bwd", "k_fwd_chunk_tc", "k_fwd_out_tc", "k_fwd_buf_y",
@@ -315,6 +311,10 @@ void prof_collect_locked() {
   g_prof.pending = 0;
 }
 
+}  // namespace
+
+namespace atlas {
+
 int prof_begin(int kid, cudaStream_t st) {
   std::lock_guard<std::mutex> lk(g_prof.mu);
   g_prof.launches++;
@@ -331,30 +331,7 @@ void prof_end(int slot, cudaStream_t st) {
   cudaEventRecord(g_prof.ev[2 * slot + 1], st);
 }
 
-#define LAUNCH_CHECK()                                              \
-  do {                                                              \
-    if (cudaGetLastError() != cudaSuccess) return ATLAS_ERR_LAUNCH; \
-  } while (0)
 
-// Launch with an explicit thread count: LAUNCH_T(id, kernel, grid, threads, smem, stream, args...)
-#define LAUNCH_T(KID, KERNEL, GRID, THREADS, SMEM, STREAM, ...)   \
-  do {                                                            \
-    const int slot_ = prof_begin(KID, STREAM);                    \
-    KERNEL<<<GRID, THREADS, SMEM, STREAM>>>(__VA_ARGS__);         \
-    LAUNCH_CHECK();                                               \
-    prof_end(slot_, STREAM);                                      \
-  } while (0)
-
-// Launch `kernel` with accounting: LAUNCH(id, kernel, grid, smem, stream, args...)
-#define LAUNCH(KID, KERNEL, GRID, SMEM, STREAM, ...)              \
-  do {                                                            \
-    const int slot_ = prof_begin(KID, STREAM);                    \
-    KERNEL<<<GRID, kThreads, SMEM, STREAM>>>(__VA_ARGS__);        \
-    LAUNCH_CHECK();                                               \
-    prof_end(slot_, STREAM);                                      \
-  } while (0)
-
-// Sequential chunk scans: float4 per thread when the state size allows it.
 int sm_count() {
   static int cached[64] = {0};
   int dev = 0;
@@ -367,6 +344,10 @@ int sm_count() {
   }
   return cached[dev];
 }
+
+}  // namespace atlas
+
+namespace {
 
 // One resident wave of tc::k_{fwd,bwd}_scan_tc: F groups of 8 elements per thread, F the smallest of
 // 1, 2, 4 that covers the units (rounds of F = 4 beyond that).
