@@ -115,6 +115,19 @@ def lib():
         L.atlas_affine_scan_forward.restype = ctypes.c_int
         L.atlas_affine_scan_backward.argtypes = [_vp] * 7 + [i64, i64, ci, ci, ci, _vp]
         L.atlas_affine_scan_backward.restype = ctypes.c_int
+        L.atlas_sscan_workspace.argtypes = [ctypes.c_char_p, sz, sz, sz]
+        L.atlas_sscan_workspace.restype = ctypes.c_int
+        L.atlas_sscan_forward.argtypes = [ctypes.c_char_p, _vp]
+        L.atlas_sscan_forward.restype = ctypes.c_int
+        L.atlas_sscan_backward.argtypes = [ctypes.c_char_p, _vp]
+        L.atlas_sscan_backward.restype = ctypes.c_int
+        L.atlas_causal_conv_forward.argtypes = [_vp, i64, i64] + [_vp] * 6 + [ci] * 3 + [i64] * 3 + [_vp]
+        L.atlas_causal_conv_forward.restype = ctypes.c_int
+        L.atlas_causal_conv_scratch.argtypes = [i64, i64, i64, ci]
+        L.atlas_causal_conv_scratch.restype = ctypes.c_size_t
+        L.atlas_causal_conv_backward.argtypes = ([_vp, i64, i64] + [_vp] * 5 + [i64, i64] + [_vp] * 6
+                                                 + [ctypes.c_size_t] + [ci] * 3 + [i64] * 3 + [_vp])
+        L.atlas_causal_conv_backward.restype = ctypes.c_int
         L.atlas_mem_read_status.argtypes = [_vp, _vp]
         L.atlas_mem_read_status.restype = ctypes.c_int
         L.atlas_mem_selftest_wait_timeout.argtypes = [_vp, ctypes.c_int, _vp]

@@ -406,6 +406,63 @@ int atlas_omega_store_backward(const float* beta, const void* surprise, const fl
                                float* d_keep, float* d_last_momentum, float* d_last_update, float* d_buf_in,
                                int64_t B, int64_t T, int64_t D, int window, int dtype_io, void* stream);
 
+/* ---- selective state space scan (no reference counterpart: its recurrences carry one scalar gate
+ * per step) ------------------------------------------------------------------------------------
+ * Per batch row b, channel d of group g = d / (D / G) and state n, over T steps:
+ *   dt_t = softplus(delta_t + bias) (softplus 0: delta_t + bias),   a_t = exp(dt_t A[d,n]),
+ *   h_t = a_t h_{t-1} + dt_t u_t B_t[g,n],  h_0 = h0 (NULL: zeros),
+ *   out_t = (sum_n C_t[g,n] h_t + Dskip u_t) silu(z_t)   (Dskip, z NULL: left out).
+ * u, delta, z, Bm, Cm, dout are in dtype_io with element strides for batch (_sb), step (_st) and, for
+ * Bm / Cm, group (_sg); channels and states are dense. All other arrays are dense: A [D,N], Dskip, bias [D],
+ * h0, hT and their gradients [B,D,N] in fp32; out, du, ddelta, dz [B,T,D] and dB, dC [B,T,G,N] in dtype_io.
+ * len [B] (int32, NULL: T): steps at or past a row's length leave the state alone, give out = 0 and
+ * zero gradients, and are not read. 1 <= N <= 64, D a multiple of G. */
+typedef struct AtlasSelScan {
+  int64_t B, T;
+  int32_t D, N, G;
+  int32_t softplus;
+  int32_t dtype_io;
+  int32_t chunk;    /* steps per time chunk, a multiple of 32; 0: library default */
+  const void *u, *delta, *z, *Bm, *Cm;
+  int64_t u_sb, u_st, delta_sb, delta_st, z_sb, z_st, B_sb, B_st, B_sg, C_sb, C_st, C_sg;
+  const float *A, *Dskip, *bias, *h0;
+  const int32_t* len;
+  void* out;
+  float* hT;
+  void* saved;      /* states kept for the backward (NULL: none is taken) */
+  void* scratch;    /* of atlas_sscan_workspace's size for the call */
+  size_t saved_bytes, scratch_bytes;
+  /* backward only; dhT NULL: zeros; dB with dC, dD, dbias, dh0 NULL: not wanted */
+  const void* dout;
+  int64_t dout_sb, dout_st;
+  const float* dhT;
+  void *du, *ddelta, *dz, *dB, *dC;
+  float *dA, *dD, *dbias, *dh0;
+} AtlasSelScan;
+/* Bytes of `saved`, and of `scratch` for a forward and a backward call, from the sizes. */
+int atlas_sscan_workspace(const AtlasSelScan* a, size_t* saved, size_t* fwd_scratch, size_t* bwd_scratch);
+int atlas_sscan_forward(const AtlasSelScan* a, void* stream);
+/* Takes the forward's inputs and `saved`. */
+int atlas_sscan_backward(const AtlasSelScan* a, void* stream);
+
+/* Causal depthwise convolution over T steps with its activation and a carried state:
+ *   y[b,t,c] = act(bias[c] + sum_{j<K} w[c,j] x[b, t + j - (K-1), c]),
+ * x at steps -(K-1) .. -1 from init [B,K-1,C] (NULL: zeros); silu 0: no activation. final [B,K-1,C] holds
+ * the last K-1 inputs up to the row's length. x has element strides x_sb, x_st (channels dense); w [C,K],
+ * bias [C] (NULL: 0) are fp32; the other arrays are dense, in dtype_io. len as above (y = 0 past it). 2 <= K <= 8. */
+int atlas_causal_conv_forward(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias,
+                              const void* init, const int32_t* len, void* y, void* final_state, int K, int silu,
+                              int dtype_io, int64_t B, int64_t T, int64_t C, void* stream);
+/* Its backward: dy [B,T,C] with strides, d_final [B,K-1,C] (NULL: zeros); dx [B,T,C], d_init [B,K-1,C] (NULL: not
+ * wanted) in dtype_io, dw [C,K] and dbias [C] (NULL: not wanted) in fp32. scratch:
+ * atlas_causal_conv_scratch(B, T, C, K) bytes. */
+size_t atlas_causal_conv_scratch(int64_t B, int64_t T, int64_t C, int K);
+int atlas_causal_conv_backward(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias,
+                               const void* init, const int32_t* len, const void* dy, int64_t dy_sb, int64_t dy_st,
+                               const void* d_final, void* dx, void* d_init, float* dw, float* dbias, void* scratch,
+                               size_t scratch_bytes, int K, int silu, int dtype_io, int64_t B, int64_t T, int64_t C,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif
