@@ -51,28 +51,110 @@ __device__ __forceinline__ f2 ex2_2(f2 x) {
 __device__ __forceinline__ float softplus(float x) {
   const float e = ex2(-fabsf(x) * kLog2e);
   const float s = e * rcp(2.f + e), q = s * s;
-  float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
-  p = fmaf(p, q, 1.f / 9.f);
-  p = fmaf(p, q, 1.f / 7.f);
-  p = fmaf(p, q, 1.f / 5.f);
-  p = fmaf(p, q, 1.f / 3.f);
-  p = fmaf(p, q, 1.f);
-  const float r = fmaf(2.f * s, p, fmaxf(x, 0.f));
-  return x != x ? x : r;
+  float p = fmaf(q, 2.f / 13.f, 2.f / 11.f);
+  p = fmaf(p, q, 2.f / 9.f);
+  p = fmaf(p, q, 2.f / 7.f);
+  p = fmaf(p, q, 2.f / 5.f);
+  p = fmaf(p, q, 2.f / 3.f);
+  p = fmaf(p, q, 2.f);
+  return fmaf(s, p, fmaxf(x, 0.f));  // a NaN comes through s
 }
 // 1 / (1 + e^-x); e^-x = inf gives 0.
 __device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-x * kLog2e)); }
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void from_f(float& o, float x) { o = x; }
+__device__ __forceinline__ void from_f(__nv_bfloat16& o, float x) { o = __float2bfloat16_rn(x); }
+
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 both(float x) { return pk(x, x); }
+__device__ __forceinline__ f2 rcp_2(f2 x) {
+  const float2 v = up(x);
+  return pk(rcp(v.x), rcp(v.y));
+}
+__device__ __forceinline__ f2 sigmoid_2(f2 x) { return rcp_2(add2(both(1.f), ex2_2(mul2(x, both(-kLog2e))))); }
+// softplus() of both halves: plain FMAs, whose constants are immediates (packed ones would take them from registers)
+__device__ __forceinline__ f2 softplus_2(f2 x) {
+  const float2 v = up(x);
+  return pk(softplus(v.x), softplus(v.y));
+}
+
+// Two neighbouring elements as fp32, and back.
+__device__ __forceinline__ f2 ld2(const float* p) { return *reinterpret_cast<const f2*>(p); }
+__device__ __forceinline__ f2 ld2(const __nv_bfloat16* p) {
+  const unsigned v = *reinterpret_cast<const unsigned*>(p);  // a bf16 is the high half of its fp32
+  return pk(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+__device__ __forceinline__ void st2(float* p, f2 v) { *reinterpret_cast<f2*>(p) = v; }
+__device__ __forceinline__ void st2(__nv_bfloat16* p, f2 v) {
+  const float2 x = up(v);
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x.x, x.y);
+}
+
+// SIZE (8 or 16) bytes to shared memory in the background: the first `bytes` from src, zeros behind them.
+template <int SIZE>
+__device__ __forceinline__ void cp_piece(void* dst, const void* src, int bytes) {
+  const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
+  if constexpr (SIZE == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(bytes) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(d), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// A warp's feed of [ROWS, W] tiles out of rows `stride` elements apart into shared memory, zeros past n columns and past
+// the rows left. `vec`: rows are 16-byte aligned and go by cp.async, each lane its own column piece (16 bytes, or the
+// row's 8) of every 32 / PER-th row (commit and wait are the caller's); otherwise element by element.
+template <class IO, int ROWS, int W>
+struct Feed {
+  static constexpr int E = W * (int)sizeof(IO) < 16 ? W : 16 / (int)sizeof(IO), PER = W / E, STEP = 32 / PER;
+  static_assert(W % E == 0 && E * sizeof(IO) >= 8 && PER <= 32 && 32 % PER == 0, "whole pieces");
+  const IO* p;  // vec: the lane's piece of the tile's first row of its own; else the tile's first row
+  int bytes;    // vec: of the lane's pieces; else the columns
+  __device__ __forceinline__ Feed(const IO* src, int64_t stride, int n, int vec, int lane) {
+    if (vec) {
+      const int k = n - lane % PER * E;
+      p = src + lane / PER * stride + lane % PER * E;
+      bytes = (k < 0 ? 0 : k > E ? E : k) * (int)sizeof(IO);
+      if (bytes == 0) p = src;
+    } else {
+      p = src;
+      bytes = n;
+    }
+  }
+  __device__ __forceinline__ void tile(IO* dst, int64_t stride, int rows, int vec, int lane) const {
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < ROWS; i += STEP) {
+        const int r = lane / PER + i;
+        if (ROWS % STEP != 0 && r >= ROWS) break;
+        cp_piece<E * (int)sizeof(IO)>(dst + r * W + lane % PER * E, p + i * stride, r < rows ? bytes : 0);
+      }
+    } else {
+#pragma unroll 4
+      for (int at = lane; at < ROWS * W; at += 32) {
+        const int r = at / W, c = at % W;
+        if (r < rows && c < bytes) dst[at] = p[r * stride + c];
+        else from_f(dst[at], 0.f);
+      }
+    }
+  }
+};
 
 // W neighbouring elements of one row.
 template <class IO, int W>
 struct alignas(W * sizeof(IO)) Vec {
   IO v[W];
 };
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void from_f(float& o, float x) { o = x; }
-__device__ __forceinline__ void from_f(__nv_bfloat16& o, float x) { o = __float2bfloat16_rn(x); }
-
 // Elements c .. c + W - 1 of a row, 0 where c + i >= n.
 template <class IO, int W>
 __device__ __forceinline__ Vec<IO, W> load_row(const IO* p, int c, int n, int vec) {
@@ -103,17 +185,44 @@ __device__ __forceinline__ Vec<IO, W> zero_row() {
   return r;
 }
 
-// Sums over L lanes whose index differs in the bits L/2 .. 1 times `stride`: p[i] over all of them,
-// lane k (its L-lane index) receives value k's sum in p[0]. L - 1 shuffles for L values.
-template <int L, int STRIDE>
-__device__ __forceinline__ void reduce_scatter(float* p, int lane) {
+// Sums of V values over L lanes (index bits of weight STRIDE, 2 STRIDE, ..): the lane of L-lane index k keeps values
+// k V/L .. in p[0 .. V/L - 1]. V - V/L exchanges instead of V log2(L).
+template <int V, int L, int STRIDE>
+__device__ __forceinline__ void reduce_part(float* p, int lane) {
+  static_assert(V >= L, "a value for every lane");
+  int n = V;
+#pragma unroll
+  for (int o = L / 2; o >= 1; o >>= 1) {
+    n >>= 1;
+    const bool hi = lane & (o * STRIDE);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i)
+      if (i < n) {
+        const float keep = hi ? p[i + n] : p[i], send = hi ? p[i] : p[i + n];
+        p[i] = keep + __shfl_xor_sync(0xffffffffu, send, o * STRIDE);
+      }
+  }
+}
+// The same over V pairs, added two at a time; the last halving splits a pair where L = 2 V (then p[0]'s low half).
+template <int V, int L, int STRIDE>
+__device__ __forceinline__ void reduce_pairs(f2* p, int lane) {
+  static_assert(2 * V >= L, "a value for every lane");
+  int n = V;
 #pragma unroll
   for (int o = L / 2; o >= 1; o >>= 1) {
     const bool hi = lane & (o * STRIDE);
+    if (n > 1) {
+      n >>= 1;
 #pragma unroll
-    for (int i = 0; i < o; ++i) {
-      const float keep = hi ? p[i + o] : p[i], send = hi ? p[i] : p[i + o];
-      p[i] = keep + __shfl_xor_sync(0xffffffffu, send, o * STRIDE);
+      for (int i = 0; i < (V + 1) / 2; ++i)
+        if (i < n) {
+          const f2 keep = hi ? p[i + n] : p[i], send = hi ? p[i] : p[i + n];
+          p[i] = add2(keep, __shfl_xor_sync(0xffffffffu, send, o * STRIDE));
+        }
+    } else {
+      const float2 v = up(p[0]);
+      const float keep = hi ? v.y : v.x, send = hi ? v.x : v.y;
+      p[0] = both(keep + __shfl_xor_sync(0xffffffffu, send, o * STRIDE));
     }
   }
 }

@@ -12,64 +12,63 @@ namespace {
 
 constexpr size_t align_up(size_t x) { return (x + 255) & ~(size_t)255; }
 
+int mc_bwd(int np) { return np < 64 ? kMcBwd<8> : kMcBwd<64>; }
 int padded(int N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 
 struct Plan {
-  int np, spt;        // padded state count, states per lane (forward)
+  int np;             // padded state count
   int chunk, nchunk;  // time axis
 };
 
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
-// Cut of the time axis: none while the rows and channels fill the machine, else enough chunks for it.
-void cut(const AtlasSelScan* a, int64_t warps, int64_t want, Plan& p) {
-  int64_t n = warps >= want ? 1 : std::min<int64_t>((want + warps - 1) / warps, 16);
-  int64_t c = a->chunk > 0 ? a->chunk : round_up((a->T + n - 1) / n, kTT);
-  if (c < 8 * kTT && a->chunk <= 0) c = 8 * kTT;
+int tiles_of(const AtlasSelScan* a, int np, int mc) {  // channel tiles (CTAs) of one group
+  const int ch = 32 / (np / kSpt) * mc * kWarps;
+  return (a->D / a->G + ch - 1) / ch;
+}
+
+// Cut of the time axis of a pass whose CTAs cover mc channels a lane and fit `resident` times on an SM. One wave of
+// CTAs where they fill the machine; the backward runs several smaller waves, whose tail weighs less against its longer
+// chunks (B 4, T 8192, D 1536, N 16: 1026 us in five waves, 1174 in one; the forward 371 in one, 389 in two), as long
+// as chunks keep 256 steps. None below 32 steps (T 512: 17 us for the forward, 25 with 64).
+void cut(const AtlasSelScan* a, int mc, int resident, int waves, Plan& p) {
+  p.np = padded(a->N);
+  const int64_t ctas = a->B * a->G * tiles_of(a, p.np, mc), wave = (int64_t)sm_count() * resident;
+  const int64_t fill = std::max<int64_t>(1, wave / ctas), many = std::max<int64_t>(1, waves * wave / ctas);
+  auto steps = [&](int64_t n) { return (a->T + n - 1) / n; };
+  int64_t c = std::max(steps(many), std::min<int64_t>(256, steps(fill)));
+  if (waves > 1 && wave / ctas < 1) c = a->T;
+  c = a->chunk > 0 ? a->chunk : round_up(std::max<int64_t>(c, 32), kTT);
   c = std::min<int64_t>(c, round_up(a->T, kTT));
   p.chunk = (int)std::min<int64_t>(c, (int64_t)1 << 30);
   p.nchunk = (int)((a->T + p.chunk - 1) / p.chunk);
 }
-
 Plan fwd_plan(const AtlasSelScan* a) {
   Plan p;
-  p.np = padded(a->N);
-  const int64_t sms = 148;
-  const int64_t w4 = (int64_t)a->B * a->D * (p.np / 4) / 32;
-  p.spt = w4 >= sms * 8 ? 4 : 2;
-  int64_t want = sms * 6;
-  cut(a, std::max<int64_t>(1, p.spt == 4 ? w4 : 2 * w4), want, p);
+  cut(a, kMcFwd, kFwdCtas, 1, p);
   return p;
 }
 Plan bwd_plan(const AtlasSelScan* a) {
   Plan p;
-  p.np = padded(a->N);
-  p.spt = 2;
-  const int64_t w = std::max<int64_t>(1, (int64_t)a->B * a->D * (p.np / 2) / 32);
-  int64_t want = 148 * 8;
-  cut(a, w, want, p);
+  cut(a, mc_bwd(padded(a->N)), kBwdCtas, 5, p);
   return p;
 }
 
 bool sizes_ok(const AtlasSelScan* a) {
   return a && a->B >= 1 && a->T >= 1 && a->D >= 1 && a->N >= 1 && a->N <= 64 && a->G >= 1 && a->D % a->G == 0 &&
-         (a->dtype_io == ATLAS_F32 || a->dtype_io == ATLAS_BF16) && a->chunk >= 0 && a->chunk % kTT == 0 &&
+         (a->dtype_io == ATLAS_F32 || a->dtype_io == ATLAS_BF16) && a->chunk >= 0 && a->chunk % 32 == 0 &&
          a->B <= (1 << 24) && a->T <= ((int64_t)1 << 40) &&
          a->B * (int64_t)a->D * (a->N / 4 + 8) < ((int64_t)1 << 36);
 }
 bool inputs_ok(const AtlasSelScan* a) { return a->u && a->delta && a->Bm && a->Cm && a->A; }
 
 size_t saved_bytes(const AtlasSelScan* a) {
-  return (size_t)a->B * ((a->T + kSaveSteps - 1) / kSaveSteps) * a->D * padded(a->N) * sizeof(float);
+  return (size_t)a->B * ((a->T + kTT - 1) / kTT) * a->D * padded(a->N) * sizeof(float);
 }
 size_t ends_bytes(const AtlasSelScan* a, const Plan& p) {
   if (p.nchunk == 1) return 0;
   const size_t rows = (size_t)a->B * p.nchunk * a->D;
   return align_up(rows * p.np * sizeof(float)) + align_up(rows * sizeof(float));
-}
-int bwd_tiles(const AtlasSelScan* a, int np) {  // channel tiles of one group
-  const int ch = kBwdThr / (np / 2);
-  return (a->D / a->G + ch - 1) / ch;
 }
 struct BwdLayout {
   size_t dbc, dA, dD, ends, total;
@@ -78,7 +77,7 @@ BwdLayout bwd_layout(const AtlasSelScan* a, const Plan& p) {
   BwdLayout L;
   size_t at = 0;
   L.dbc = at;
-  at += align_up((size_t)a->G * bwd_tiles(a, p.np) * a->B * a->T * 2 * p.np * sizeof(float));
+  at += align_up((size_t)a->G * tiles_of(a, p.np, mc_bwd(p.np)) * a->B * a->T * 2 * p.np * sizeof(float));
   L.dA = at;
   at += align_up((size_t)a->B * p.nchunk * a->D * p.np * sizeof(float));
   L.dD = at;
@@ -106,33 +105,54 @@ ScanArgs pack(const AtlasSelScan* a, const Plan& p) {
 bool wide(const void* p, int64_t sb, int64_t st, int size, int W) {
   return !p || ((uintptr_t)p % (size_t)(W * size) == 0 && sb % W == 0 && st % W == 0);
 }
-void alignment(const AtlasSelScan* a, ScanArgs& s, int W, bool bwd) {
-  const int size = a->dtype_io == ATLAS_BF16 ? 2 : 4;
-  s.vec = wide(a->u, a->u_sb, a->u_st, size, W) && wide(a->delta, a->delta_sb, a->delta_st, size, W) &&
-          wide(a->z, a->z_sb, a->z_st, size, W) && wide(a->out, a->D, a->D, size, W) &&
-          (a->G == 1 || a->D / a->G % W == 0);
-  if (bwd)
-    s.vec = s.vec && wide(a->dout, a->dout_sb, a->dout_st, size, W) && wide(a->du, a->D, a->D, size, W) &&
-            wide(a->ddelta, a->D, a->D, size, W) && wide(a->dz, a->D, a->D, size, W);
-  s.vecbc = wide(a->Bm, a->B_sb, a->B_st, size, 4) && wide(a->Cm, a->C_sb, a->C_st, size, 4) &&
-            (a->G == 1 || (a->B_sg % 4 == 0 && a->C_sg % 4 == 0));
+// vec, vecbc: 16-byte pieces of the rows read, of B and C (one token: 4 elements of them); pair: two elements of the rows written.
+void alignment(const AtlasSelScan* a, ScanArgs& s, int bc) {
+  const int size = a->dtype_io == ATLAS_BF16 ? 2 : 4, E = 16 / size;
+  const int64_t dg = a->G == 1 ? 0 : a->D / a->G;
+  s.vec = wide(a->u, a->u_sb, a->u_st, size, E) && wide(a->delta, a->delta_sb, a->delta_st, size, E) &&
+          wide(a->z, a->z_sb, a->z_st, size, E) && wide(a->dout, a->dout_sb, a->dout_st, size, E) && dg % E == 0;
+  s.pair = wide(a->out, a->D, a->D, size, 2) && wide(a->du, a->D, a->D, size, 2) &&
+           wide(a->ddelta, a->D, a->D, size, 2) && wide(a->dz, a->D, a->D, size, 2) && dg % 2 == 0;
+  s.vecbc = wide(a->Bm, a->B_sb, a->B_st, size, bc) && wide(a->Cm, a->C_sb, a->C_st, size, bc) &&
+            (a->G == 1 || (a->B_sg % bc == 0 && a->C_sg % bc == 0));
 }
 
-template <class IO, int NP, int SPT>
-int fwd_t(const AtlasSelScan* a, ScanArgs s, cudaStream_t st) {
-  constexpr int CH = kFwdThr / (NP / SPT);
-  alignment(a, s, RowTile<IO, CH, kFwdThr, kTT>::W, false);
-  const int64_t gx = a->B * a->G * ((a->D / a->G + CH - 1) / CH);
-  if (gx > 0x7fffffff || s.nchunk > 65535) return ATLAS_ERR_UNSUPPORTED;
-  if (s.nchunk > 1)
-    LAUNCH_T(KID_SSCAN_ENDS, (k_sscan_fwd<IO, NP, SPT, true>), dim3((unsigned)gx, s.nchunk - 1), kFwdThr, 0, st, s);
-  LAUNCH_T(KID_SSCAN_FWD, (k_sscan_fwd<IO, NP, SPT, false>), dim3((unsigned)gx, s.nchunk), kFwdThr, 0, st, s);
+// A walking kernel over (batch x groups x channel tiles, chunks) with its warps' shared memory.
+template <class K>
+int walk(int kid, K kernel, const AtlasSelScan* a, const ScanArgs& s, int tiles, int chunks, int bytes, cudaStream_t st) {
+  const int64_t gx = a->B * a->G * tiles;
+  if (gx > 0x7fffffff || chunks > 65535) return ATLAS_ERR_UNSUPPORTED;
+  if (bytes > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return ATLAS_ERR_LAUNCH;
+  LAUNCH_T(kid, kernel, dim3((unsigned)gx, chunks), 32 * kWarps, bytes, st, s);
   return ATLAS_OK;
+}
+
+template <int NP, bool BACK>
+int carry(const AtlasSelScan* a, const ScanArgs& s, cudaStream_t st) {
+  const int64_t n = a->B * a->D * (NP / 4), grid = (n + kCarryThr - 1) / kCarryThr;
+  if (grid > 0x7fffffff) return ATLAS_ERR_UNSUPPORTED;
+  LAUNCH_T(KID_SSCAN_CARRY, (k_sscan_carry<NP, BACK>), dim3((unsigned)grid), kCarryThr, 0, st, s);
+  return ATLAS_OK;
+}
+
+template <class IO, int NP, bool Z>
+int fwd_t(const AtlasSelScan* a, ScanArgs s, cudaStream_t st) {
+  const int tiles = tiles_of(a, NP, kMcFwd);
+  alignment(a, s, 16 / (int)sizeof(IO));
+  if (s.nchunk > 1) {
+    if (const int rc = walk(KID_SSCAN_ENDS, k_sscan_fwd<IO, NP, true, false>, a, s, tiles, s.nchunk - 1,
+                            kWarps * (int)sizeof(FwdSmem<IO, NP, true, false>), st))
+      return rc;
+    if (const int rc = carry<NP, false>(a, s, st)) return rc;
+  }
+  return walk(KID_SSCAN_FWD, k_sscan_fwd<IO, NP, false, Z>, a, s, tiles, s.nchunk,
+              kWarps * (int)sizeof(FwdSmem<IO, NP, false, Z>), st);
 }
 
 template <class IO, int NP>
 int step_t(const AtlasSelScan* a, ScanArgs s, cudaStream_t st) {
-  alignment(a, s, 1, false);
+  alignment(a, s, 4);
   const int vec4 = a->N % 4 == 0 && (uintptr_t)a->A % 16 == 0 && (uintptr_t)a->h0 % 16 == 0 &&
                    (uintptr_t)a->hT % 16 == 0;
   const int64_t per = kStepThr / (NP / 4), grid = (a->B * a->D + per - 1) / per;
@@ -141,29 +161,24 @@ int step_t(const AtlasSelScan* a, ScanArgs s, cudaStream_t st) {
   return ATLAS_OK;
 }
 
-template <class IO, int NP>
+template <class IO, int NP, bool Z>
 int bwd_t(const AtlasSelScan* a, ScanArgs s, const BwdLayout& L, cudaStream_t st) {
-  constexpr int CH = BwdSmem<NP>::CH, FCH = kFwdThr / (NP / 2);
-  const int64_t dg = a->D / a->G, tiles = (dg + CH - 1) / CH, gx = a->B * a->G * tiles;
   const int64_t rows = a->B * a->T;
-  if (gx > 0x7fffffff || s.nchunk > 65535) return ATLAS_ERR_UNSUPPORTED;
+  const int tiles = tiles_of(a, NP, kMcBwd<NP>);
+  alignment(a, s, 16 / (int)sizeof(IO));
   if (s.nchunk > 1) {
-    ScanArgs e = s;
-    alignment(a, e, RowTile<IO, FCH, kFwdThr, kTT>::W, true);
-    const int64_t ex = a->B * a->G * ((dg + FCH - 1) / FCH);
-    if (ex > 0x7fffffff) return ATLAS_ERR_UNSUPPORTED;
-    LAUNCH_T(KID_SSCAN_BWD_ENDS, (k_sscan_bwd_ends<IO, NP, 2>), dim3((unsigned)ex, s.nchunk - 1), kFwdThr, 0, st, e);
+    if (const int rc = walk(KID_SSCAN_BWD_ENDS, k_sscan_bwd_ends<IO, NP, Z>, a, s, tiles, s.nchunk - 1,
+                            kWarps * (int)sizeof(EndsSmem<IO, NP, Z>), st))
+      return rc;
+    if (const int rc = carry<NP, true>(a, s, st)) return rc;
   }
-  alignment(a, s, RowTile<IO, CH, kBwdThr, kTT>::W, true);
-  if (cudaFuncSetAttribute(k_sscan_bwd<IO, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdSmem<NP>::bytes) !=
-      cudaSuccess)
-    return ATLAS_ERR_LAUNCH;
-  LAUNCH_T(KID_SSCAN_BWD, (k_sscan_bwd<IO, NP>), dim3((unsigned)gx, s.nchunk), kBwdThr, BwdSmem<NP>::bytes, st, s);
-  if (s.dbc) {
+  if (const int rc = walk(KID_SSCAN_BWD, k_sscan_bwd<IO, NP, Z>, a, s, tiles, s.nchunk, (int)sizeof(BwdSmem<IO, NP, Z>), st))
+    return rc;
+  if (a->dB) {
     const int64_t blocks = (rows * 2 * NP / 4 + 255) / 256;
     if (blocks > 0x7fffffff || a->G > 65535) return ATLAS_ERR_UNSUPPORTED;
     LAUNCH_T(KID_SSCAN_DBC, (k_sscan_dbc<IO, NP>), dim3((unsigned)blocks, a->G), 256, 0, st, s.dbc, (IO*)a->dB,
-             (IO*)a->dC, rows, a->N, a->G, (int)tiles);
+             (IO*)a->dC, rows, a->N, a->G, tiles_of(a, NP, kMcBwd<NP>));
   }
   const int64_t n = (int64_t)a->D * NP + 2 * (int64_t)a->D;
   LAUNCH_T(KID_SSCAN_DA, k_sscan_dA, dim3((unsigned)((n + 255) / 256)), 256, 0, st, s.part_dA, s.part_dD, a->dA, a->dD,
@@ -181,24 +196,20 @@ int fwd_io(const AtlasSelScan* a, const Plan& p, const ScanArgs& s, cudaStream_t
       default: return step_t<IO, 64>(a, s, st);
     }
   }
-  switch (p.np * 10 + p.spt) {
-    case 82: return fwd_t<IO, 8, 2>(a, s, st);
-    case 84: return fwd_t<IO, 8, 4>(a, s, st);
-    case 162: return fwd_t<IO, 16, 2>(a, s, st);
-    case 164: return fwd_t<IO, 16, 4>(a, s, st);
-    case 322: return fwd_t<IO, 32, 2>(a, s, st);
-    case 324: return fwd_t<IO, 32, 4>(a, s, st);
-    case 642: return fwd_t<IO, 64, 2>(a, s, st);
-    default: return fwd_t<IO, 64, 4>(a, s, st);
+  switch (p.np) {
+    case 8: return a->z ? fwd_t<IO, 8, true>(a, s, st) : fwd_t<IO, 8, false>(a, s, st);
+    case 16: return a->z ? fwd_t<IO, 16, true>(a, s, st) : fwd_t<IO, 16, false>(a, s, st);
+    case 32: return a->z ? fwd_t<IO, 32, true>(a, s, st) : fwd_t<IO, 32, false>(a, s, st);
+    default: return a->z ? fwd_t<IO, 64, true>(a, s, st) : fwd_t<IO, 64, false>(a, s, st);
   }
 }
 template <class IO>
 int bwd_io(const AtlasSelScan* a, const Plan& p, const ScanArgs& s, const BwdLayout& L, cudaStream_t st) {
   switch (p.np) {
-    case 8: return bwd_t<IO, 8>(a, s, L, st);
-    case 16: return bwd_t<IO, 16>(a, s, L, st);
-    case 32: return bwd_t<IO, 32>(a, s, L, st);
-    default: return bwd_t<IO, 64>(a, s, L, st);
+    case 8: return a->z ? bwd_t<IO, 8, true>(a, s, L, st) : bwd_t<IO, 8, false>(a, s, L, st);
+    case 16: return a->z ? bwd_t<IO, 16, true>(a, s, L, st) : bwd_t<IO, 16, false>(a, s, L, st);
+    case 32: return a->z ? bwd_t<IO, 32, true>(a, s, L, st) : bwd_t<IO, 32, false>(a, s, L, st);
+    default: return a->z ? bwd_t<IO, 64, true>(a, s, L, st) : bwd_t<IO, 64, false>(a, s, L, st);
   }
 }
 
@@ -241,7 +252,7 @@ int atlas_sscan_backward(const AtlasSelScan* a, void* stream) {
   ScanArgs s = pack(a, p);
   char* w = (char*)a->scratch;
   s.hsave = (float*)a->saved;
-  s.dbc = a->dB ? (float*)(w + L.dbc) : nullptr;
+  s.dbc = (float*)(w + L.dbc);
   s.part_dA = (float*)(w + L.dA);
   s.part_dD = (float*)(w + L.dD);
   if (p.nchunk > 1) {

@@ -6,27 +6,36 @@
 // the floor: 16 per cycle and SM on the special-function unit, against about 20 bytes of traffic
 // per (token, channel).
 //
-// Layout of the work: a channel's states lie across LPC = NP / SPT lanes, SPT states a lane (NP: the
-// state count padded to a power of two with A = B = C = 0 columns, whose states stay 0). A CTA owns
-// kThr / LPC neighbouring channels and walks the time axis in tiles of kTT steps: the tile's rows
-// are read once, coalesced, one tile ahead of their use; dt and dt u go through shared memory
-// as fp32, B and C too (shared by all channels of the tile); the walk itself runs in
-// registers; the sums over a channel's lanes are transposed reductions over LPC steps at
-// a time (LPC - 1 shuffles give LPC steps' sums, one per lane). Lengths: a step at or past its row's
-// length has dt = 0 (a = 1, no input) and writes 0.
+// Layout of the work: a channel's states lie across LPC = NP / kSpt lanes (NP: the state count padded to a power of two
+// with A = B = C = 0 columns, whose states stay 0), and a lane holds the states of MC neighbouring channels: a load from
+// shared memory returns 4 bytes a lane and cycle, so B and C serve the lane's MC channels, dt and dt u its kSpt states
+// (one channel a lane cost 3.5 load cycles of the SM a state-update of a warp, above the exponential's 2). A
+// warp walks the time axis in tiles of kTT steps. Everything is the warp's own, so a tile costs no block barrier: rows
+// arrive by cp.async one tile ahead and become dt, dt u, B, C in fp32; arithmetic is packed fp32 pairs over
+// neighbouring states; the sums over a channel's lanes are transposed reductions (LPC values over LPC lanes in
+// LPC - 1 exchanges). Lengths: a step at or past its row's length is not read and writes 0.
 //
 // When the rows and channels do not fill the machine, the time axis is cut into chunks: a first
-// pass leaves each chunk's own end state (from zero) and its sum of dt, the second starts
-// every chunk from h = sum over earlier chunks, each decayed by exp(A sum dt). That pays the
-// exponentials twice.
+// pass leaves each chunk's own end state (from zero) and its sum of dt, k_sscan_carry turns them into the states
+// that enter the chunks (each earlier one decayed by exp(A sum dt)), and the pass over the outputs starts from those.
+// That pays the exponentials twice.
 #pragma once
 #include "row_ops.cuh"
 
 namespace atlas {
 namespace ss {
 
-constexpr int kTT = 32;       // steps per tile
-constexpr int kSaveSteps = 16;  // training: the state before every 16th step is kept for the backward
+// Channels per lane, forward and backward. Forward 4: fewer shared-memory loads and instructions a state (measured at
+// B 4, T 8192, D 1536, N 16, bf16: 371 us, against 391-425 for 2 with as many or more warps). Backward 2: the states of
+// kTT steps stay in 168 registers (1103 us; 4 needs 255 registers: 1151-1275). Wide states take 4: 2 would leave a
+// warp less than 16 bytes of a row.
+constexpr int kMcFwd = 4;
+template <int NP>
+constexpr int kMcBwd = NP < 64 ? 2 : 4;
+constexpr int kTT = 8;     // steps per tile; training keeps the state before each
+constexpr int kSpt = 4;    // states per lane
+constexpr int kWarps = 4;   // per CTA
+constexpr int kFwdCtas = 4, kBwdCtas = 3;  // resident on an SM (registers: 128 and 168 a thread)
 
 struct ScanArgs {
   const void *u, *delta, *z, *Bm, *Cm, *dout;
@@ -36,7 +45,7 @@ struct ScanArgs {
   const int* len;
   void* out;       // [B, T, Dm]
   float* hT;       // [B, Dm, N]
-  float* hsave;    // [B, ceil(T / kSaveSteps), Dm, NP]
+  float* hsave;    // [B, ceil(T / kTT), Dm, NP]
   float* part_h;   // [B, nchunk, Dm, NP]  chunk end states (backward: start adjoints)
   float* part_dt;  // [B, nchunk, Dm]      chunk sums of dt
   // backward
@@ -49,235 +58,349 @@ struct ScanArgs {
   int64_t T;
   int Bsz, Dm, N, G, softplus, chunk, nchunk;  // chunk: steps per chunk, a multiple of kTT
   int vec;   // every row tensor allows whole-vector accesses (16 bytes or the thread's share)
-  int vecbc; // B and C allow 4-element accesses
+  int vecbc; // B and C allow 16-byte (backward: 4-element) accesses
+  int pair;  // the output's rows allow two-element accesses at even channels
 };
 
-// ---- forward --------------------------------------------------------------
-constexpr int kFwdThr = 128;
+// ---- shared by the passes -------------------------------------------------
+template <int NP, int MC>
+struct Shape {
+  static constexpr int LPC = NP / kSpt;      // lanes across a channel's states
+  static constexpr int Q = 32 / LPC;         // channel groups in a warp
+  static constexpr int CH = Q * MC;          // channels of a warp
+  static constexpr int PC = CH / 2 < 32 ? CH / 2 : 32;  // row phases: a lane takes two channels of a row ..
+  static constexpr int PR = 32 / PC;         // .. PR rows at a time
+  static constexpr int SY = LPC > MC ? LPC / MC : 1;    // steps per reduction over a channel's lanes
+  static constexpr int SB = Q > kSpt ? Q / kSpt : 1;    // steps per reduction over the warp's channel groups
+  static_assert(PC * 2 == CH && kTT % PR == 0 && SY <= kTT && SB <= kTT, "tile");
+};
 
-// Row tile of a CTA: R rows of CH channels; the thread's elements are W neighbours of one or more rows.
-template <class IO, int CH, int THR, int ROWS>
-struct RowTile {
-  static constexpr int kEach = ROWS * CH / THR;                 // elements per thread
-  static constexpr int kMax = 16 / (int)sizeof(IO);
-  static constexpr int W = kEach < kMax ? (kEach < CH ? kEach : CH) : (kMax < CH ? kMax : CH);
-  static constexpr int kVecs = kEach / W;
-  static constexpr int kCols = CH / W, kRowStep = THR / kCols;
-  static_assert(kEach >= 1 && kVecs * W == kEach && kCols * W == CH && kRowStep * kVecs == ROWS, "row tile");
+// A warp's place in the problem.
+template <int CH>
+struct Place {
+  int b, g, nc, tile;  // nc: channels it really has; tile: the CTA's channel tile index over all groups
+  int64_t d0, len;
+  __device__ Place(const ScanArgs& a, int warp) {
+    const int Dg = a.Dm / a.G, tiles = (Dg + CH * kWarps - 1) / (CH * kWarps);
+    b = blockIdx.x / (tiles * a.G);
+    tile = blockIdx.x - b * tiles * a.G;
+    g = tile / tiles;
+    const int c = ((tile - g * tiles) * kWarps + warp) * CH;
+    nc = Dg - c < CH ? (Dg - c < 0 ? 0 : Dg - c) : CH;
+    d0 = (int64_t)g * Dg + (nc ? c : 0);
+    len = row_len(a.len, b, a.T);
+  }
+};
+
+// A lane's MC x kSpt block of per-(channel, state) values, as pairs over neighbouring states.
+template <int MC>
+struct Block {
+  f2 v[MC][kSpt / 2];
+  // value(c, i) of the lane's channel c and state i
+  template <class F>
+  __device__ __forceinline__ void fill(F value) {
+#pragma unroll
+    for (int c = 0; c < MC; ++c)
+#pragma unroll
+      for (int p = 0; p < kSpt / 2; ++p) v[c][p] = pk(value(c, 2 * p), value(c, 2 * p + 1));
+  }
+  __device__ __forceinline__ float at(int c, int i) const {
+    const float2 x = up(v[c][i / 2]);
+    return i % 2 ? x.y : x.x;
+  }
+};
+
+// A [Dm, N] in units of log2.
+template <int MC, int CH>
+__device__ __forceinline__ void load_A(const ScanArgs& a, const Place<CH>& w, int c4, int n4, Block<MC>& A) {
+  A.fill([&](int c, int i) {
+    return c4 + c < w.nc && n4 + i < a.N ? a.A[(w.d0 + c4 + c) * a.N + n4 + i] * kLog2e : 0.f;
+  });
+}
+// A state [B, Dm, N] (null: zeros).
+template <int MC, int CH>
+__device__ __forceinline__ void load_state(const ScanArgs& a, const Place<CH>& w, const float* s, int c4, int n4,
+                                           Block<MC>& h) {
+  h.fill([&](int c, int i) {
+    return s && c4 + c < w.nc && n4 + i < a.N ? s[((int64_t)w.b * a.Dm + w.d0 + c4 + c) * a.N + n4 + i] : 0.f;
+  });
+}
+template <int MC, int CH>
+__device__ __forceinline__ void store_state(const ScanArgs& a, const Place<CH>& w, float* s, int c4, int n4,
+                                            const Block<MC>& h) {
+#pragma unroll
+  for (int c = 0; c < MC; ++c)
+#pragma unroll
+    for (int i = 0; i < kSpt; ++i)
+      if (c4 + c < w.nc && n4 + i < a.N) s[((int64_t)w.b * a.Dm + w.d0 + c4 + c) * a.N + n4 + i] = h.at(c, i);
+}
+// Channel rows of NP padded states (16-byte pieces).
+template <int NP, int MC>
+__device__ __forceinline__ void store_rows(float* rows, int nc, int c4, int n4, const Block<MC>& h) {
+#pragma unroll
+  for (int c = 0; c < MC; ++c)
+    if (c4 + c < nc)
+      *reinterpret_cast<ulonglong2*>(rows + (int64_t)(c4 + c) * NP + n4) = make_ulonglong2(h.v[c][0], h.v[c][1]);
+}
+template <int NP, int MC>
+__device__ __forceinline__ void load_rows(const float* rows, int nc, int c4, int n4, Block<MC>& h) {
+#pragma unroll
+  for (int c = 0; c < MC; ++c) {
+    ulonglong2 x = make_ulonglong2(0, 0);
+    if (c4 + c < nc) x = *reinterpret_cast<const ulonglong2*>(rows + (int64_t)(c4 + c) * NP + n4);
+    h.v[c][0] = x.x, h.v[c][1] = x.y;
+  }
+}
+// A lane's channels in a row of fp32, each as a pair.
+template <int MC>
+struct Chans {
+  f2 v[MC];
+  __device__ __forceinline__ explicit Chans(const float* p) {
+    if constexpr (MC == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(p);
+      v[0] = both(x.x), v[1] = both(x.y), v[2] = both(x.z), v[3] = both(x.w);
+    } else {
+      const float2 x = *reinterpret_cast<const float2*>(p);
+      v[0] = both(x.x), v[1] = both(x.y);
+    }
+  }
+};
+// A [kTT, NP] tile in fp32.
+template <class IO, int NP>
+__device__ __forceinline__ void widen(float (*dst)[NP], const IO* raw, int lane) {
+#pragma unroll
+  for (int k = 0; k < kTT * NP; k += 64) st2(&dst[0][0] + k + lane * 2, ld2(raw + k + lane * 2));
+}
+// A lane's four states in a row of fp32.
+struct States {
+  f2 v[kSpt / 2];
+  __device__ __forceinline__ explicit States(const float* p) {
+    const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(p);
+    v[0] = x.x, v[1] = x.y;
+  }
+};
+// One step of the recurrence.
+template <int MC>
+__device__ __forceinline__ void advance(Block<MC>& h, const Block<MC>& from, const Block<MC>& A, const Chans<MC>& dt,
+                                        const Chans<MC>& du, const States& B) {
+#pragma unroll
+  for (int c = 0; c < MC; ++c)
+#pragma unroll
+    for (int p = 0; p < kSpt / 2; ++p)
+      h.v[c][p] = fma2(ex2_2(mul2(A.v[c][p], dt.v[c])), from.v[c][p], mul2(du.v[c], B.v[p]));
+}
+// The lane's share of sum_n C h, per channel.
+template <int MC>
+__device__ __forceinline__ void dot(float* y, const Block<MC>& h, const States& C) {
+#pragma unroll
+  for (int c = 0; c < MC; ++c) {
+    const float2 v = up(fma2(C.v[1], h.v[c][1], mul2(C.v[0], h.v[c][0])));
+    y[c] = v.x + v.y;
+  }
+}
+// Two neighbouring elements of a row written: both where the warp's tile is whole and pairs are aligned.
+template <class IO>
+__device__ __forceinline__ void store2(IO* o, f2 v, bool whole, bool c0, bool c1) {
+  if (whole) {
+    st2(o, v);
+  } else {
+    const float2 x = up(v);
+    if (c0) from_f(o[0], x.x);
+    if (c1) from_f(o[1], x.y);
+  }
+}
+// Sum over the lanes that share the column pair of a row phase.
+template <int PC>
+__device__ __forceinline__ f2 over_rows(f2 x) {
+#pragma unroll
+  for (int o = PC; o < 32; o <<= 1) x = add2(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+
+// ---- forward --------------------------------------------------------------
+template <class IO, int NP, bool ENDS, bool Z>
+struct FwdSmem {  // one warp's
+  static constexpr int kRows = Z ? 3 : 2, kBC = ENDS ? 1 : 2, CH = Shape<NP, kMcFwd>::CH;
+  struct Raw {  // a tile as it lies in memory
+    alignas(16) IO rows[kRows][kTT][CH];  // delta, u, z
+    alignas(16) IO bc[kBC][kTT][NP];
+  };
+  Raw raw[2];
+  alignas(16) float dt[kTT][CH];
+  alignas(16) float du[kTT][CH];
+  alignas(16) float b[kTT][NP];
+  alignas(16) float c[ENDS ? 1 : kTT][NP];
+  alignas(16) float y[ENDS ? 1 : kTT][CH];
 };
 
 // grid (batch x groups x channel tiles, chunks). ENDS: only the chunk's end state and sum of dt.
-template <class IO, int NP, int SPT, bool ENDS>
-__global__ void __launch_bounds__(kFwdThr) k_sscan_fwd(const ScanArgs a) {
-  constexpr int LPC = NP / SPT, CH = kFwdThr / LPC, CPW = 32 / LPC, YS = CH + CPW, P2 = SPT / 2;
-  using RT = RowTile<IO, CH, kFwdThr, kTT>;
-  constexpr int W = RT::W, NV = RT::kVecs;
-  constexpr int BU = kTT * NP / 4 / kFwdThr > 0 ? kTT * NP / 4 / kFwdThr : 1;  // 4-state units of B per thread
-  __shared__ __align__(16) float2 s_dt[kTT][CH];
-  __shared__ __align__(16) float s_b[kTT][NP];
-  __shared__ __align__(16) float s_c[ENDS ? 1 : kTT][NP];
-  __shared__ __align__(16) float s_y[ENDS ? 1 : kTT][YS];
-  const int tid = threadIdx.x, lane = tid & 31, l = lane % LPC, ch = tid / LPC;
-  const int Dg = a.Dm / a.G, tiles = (Dg + CH - 1) / CH;
-  const int b = blockIdx.x / (tiles * a.G), gt = blockIdx.x - b * tiles * a.G;
-  const int g = gt / tiles, cbase = (gt - g * tiles) * CH;  // channel tile inside its group
-  const int chunk = blockIdx.y;
+template <class IO, int NP, bool ENDS, bool Z>
+__global__ void __launch_bounds__(32 * kWarps, kFwdCtas) k_sscan_fwd(const ScanArgs a) {
+  using SM = FwdSmem<IO, NP, ENDS, Z>;
+  constexpr int MC = kMcFwd;
+  using S = Shape<NP, MC>;
+  constexpr int LPC = S::LPC, CH = S::CH, PC = S::PC, PR = S::PR, SY = S::SY;
+  extern __shared__ __align__(16) unsigned char sm_raw[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % LPC;
+  SM& sm = reinterpret_cast<SM*>(sm_raw)[warp];
+  const Place<CH> w(a, warp);
+  if (!w.nc) return;  // warps do not wait for one another here
+  const int chunk = blockIdx.y, c4 = lane / LPC * MC, n4 = l * kSpt;
   const int64_t t_lo = (int64_t)chunk * a.chunk, t_hi = t_lo + a.chunk < a.T ? t_lo + a.chunk : a.T;
-  const int64_t len = row_len(a.len, b, a.T);
-  const int nc = Dg - cbase < CH ? Dg - cbase : CH;  // channels of this tile
-  const int64_t d0 = (int64_t)g * Dg + cbase;
-  const IO* up_ = (const IO*)a.u + b * a.u_sb + d0;
-  const IO* dp_ = (const IO*)a.delta + b * a.d_sb + d0;
-  const IO* zp_ = a.z ? (const IO*)a.z + b * a.z_sb + d0 : nullptr;
-  const IO* bp_ = (const IO*)a.Bm + b * a.B_sb + g * a.B_sg;
-  const IO* cp_ = (const IO*)a.Cm + b * a.C_sb + g * a.C_sg;
-  const int rcol = (tid % RT::kCols) * W, rrow = tid / RT::kCols;
-
-  // this lane's states: A in units of log2, the state the chunk starts from
-  const bool mine = ch < nc;
-  f2 A2[P2], h[P2];
-  {
-    float av[SPT], hv[SPT];
-#pragma unroll
-    for (int i = 0; i < SPT; ++i) {
-      const int n = l * SPT + i;
-      av[i] = mine && n < a.N ? a.A[(d0 + ch) * a.N + n] * kLog2e : 0.f;
-      hv[i] = !ENDS && mine && n < a.N && a.h0 ? a.h0[((int64_t)b * a.Dm + d0 + ch) * a.N + n] : 0.f;
+  const int64_t t_live = t_hi < w.len ? t_hi : w.len;
+  const int pc = lane % PC * 2, pr = lane / PC;
+  using Rows = Feed<IO, kTT, CH>;
+  using Cols = Feed<IO, kTT, NP>;
+  Rows fd((const IO*)a.delta + w.b * a.d_sb + t_lo * a.d_st + w.d0, a.d_st, w.nc, a.vec, lane);
+  Rows fu((const IO*)a.u + w.b * a.u_sb + t_lo * a.u_st + w.d0, a.u_st, w.nc, a.vec, lane);
+  Rows fz(Z ? (const IO*)a.z + w.b * a.z_sb + t_lo * a.z_st + w.d0 : nullptr, a.z_st, w.nc, a.vec, lane);
+  Cols fb((const IO*)a.Bm + w.b * a.B_sb + w.g * a.B_sg + t_lo * a.B_st, a.B_st, a.N, a.vecbc, lane);
+  Cols fc((const IO*)a.Cm + w.b * a.C_sb + w.g * a.C_sg + t_lo * a.C_st, a.C_st, a.N, a.vecbc, lane);
+  auto fetch = [&](int rows, int s) {  // the next tile
+    auto& r = sm.raw[s];
+    fd.tile(&r.rows[0][0][0], a.d_st, rows, a.vec, lane);
+    fu.tile(&r.rows[1][0][0], a.u_st, rows, a.vec, lane);
+    fd.p += kTT * a.d_st, fu.p += kTT * a.u_st;
+    if (Z) {
+      fz.tile(&r.rows[SM::kRows - 1][0][0], a.z_st, rows, a.vec, lane);
+      fz.p += kTT * a.z_st;
     }
-    if (!ENDS && mine)
-      for (int c = 0; c < chunk; ++c) {
-        const int64_t at = ((int64_t)b * a.nchunk + c) * a.Dm + d0 + ch;
-        const float sdt = a.part_dt[at];
-#pragma unroll
-        for (int i = 0; i < SPT; ++i) hv[i] = fmaf(ex2(av[i] * sdt), hv[i], a.part_h[at * NP + l * SPT + i]);
-      }
-#pragma unroll
-    for (int i = 0; i < P2; ++i) A2[i] = pk(av[2 * i], av[2 * i + 1]), h[i] = pk(hv[2 * i], hv[2 * i + 1]);
-  }
-  float bias[W], Dv[W];
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
-    const bool ok = rcol + i < nc;
-    bias[i] = ok && a.bias ? a.bias[d0 + rcol + i] : 0.f;
-    Dv[i] = ok && a.D ? a.D[d0 + rcol + i] : 0.f;
-  }
-  float sdt[W];
-#pragma unroll
-  for (int i = 0; i < W; ++i) sdt[i] = 0.f;
-
-  Vec<IO, W> ru[NV], rd[NV], rz[NV];
-  Vec<IO, 4> rb[BU], rc[BU];
-  auto fetch = [&](int64_t t0) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int64_t t = t0 + rrow + v * RT::kRowStep;
-      if (t < t_hi && t < len) {
-        ru[v] = load_row<IO, W>(up_ + t * a.u_st, rcol, nc, a.vec);
-        rd[v] = load_row<IO, W>(dp_ + t * a.d_st, rcol, nc, a.vec);
-        if (!ENDS && zp_) rz[v] = load_row<IO, W>(zp_ + t * a.z_st, rcol, nc, a.vec);
-      } else {
-        ru[v] = rd[v] = rz[v] = zero_row<IO, W>();
-      }
+    fb.tile(&r.bc[0][0][0], a.B_st, rows, a.vecbc, lane);
+    fb.p += kTT * a.B_st;
+    if (!ENDS) {
+      fc.tile(&r.bc[SM::kBC - 1][0][0], a.C_st, rows, a.vecbc, lane);
+      fc.p += kTT * a.C_st;
     }
-#pragma unroll
-    for (int v = 0; v < BU; ++v) {
-      const int at = tid + v * kFwdThr, tt = at / (NP / 4), n = (at % (NP / 4)) * 4;
-      rb[v] = rc[v] = zero_row<IO, 4>();
-      if (tt < kTT && t0 + tt < t_hi && t0 + tt < len) {
-        rb[v] = load_row<IO, 4>(bp_ + (t0 + tt) * a.B_st, n, a.N, a.vecbc);
-        if (!ENDS) rc[v] = load_row<IO, 4>(cp_ + (t0 + tt) * a.C_st, n, a.N, a.vecbc);
-      }
-    }
+    cp_commit();
   };
-  const int64_t nblk = (a.T + kSaveSteps - 1) / kSaveSteps;
+  int left = t_live > t_lo ? (int)(t_live - t_lo) : 0;  // steps to walk
+  if (left) fetch(left, 0);
 
-  fetch(t_lo);
-  for (int64_t t0 = t_lo; t0 < t_hi; t0 += kTT) {
-    if (t0 >= len) {  // nothing but zeros from here on (the whole CTA: len is the row's)
-      if (!ENDS) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          const int64_t t = t0 + rrow + v * RT::kRowStep;
-          if (t < t_hi)
-            store_row<IO, W>((IO*)a.out + (b * a.T + t) * a.Dm + d0, rcol, nc, a.vec, zero_row<IO, W>());
-        }
-        continue;
-      }
-      break;
-    }
-    // dt, dt u, B, C of the tile; the raw rows of u and z stay for the epilogue
-    Vec<IO, W> cu[NV], cz[NV];
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int tt = rrow + v * RT::kRowStep;
-      const bool live = t0 + tt < t_hi && t0 + tt < len;
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        float x = to_f(rd[v].v[i]) + bias[i];
-        if (a.softplus) x = softplus(x);
-        if (!live) x = 0.f;
-        sdt[i] += x;
-        s_dt[tt][rcol + i] = make_float2(x, x * to_f(ru[v].v[i]));
-      }
-      cu[v] = ru[v];
-      cz[v] = rz[v];
-    }
-#pragma unroll
-    for (int v = 0; v < BU; ++v) {
-      const int at = tid + v * kFwdThr, tt = at / (NP / 4), n = (at % (NP / 4)) * 4;
-      if (tt < kTT) {
-        *reinterpret_cast<float4*>(&s_b[tt][n]) =
-            make_float4(to_f(rb[v].v[0]), to_f(rb[v].v[1]), to_f(rb[v].v[2]), to_f(rb[v].v[3]));
-        if (!ENDS)
-          *reinterpret_cast<float4*>(&s_c[tt][n]) =
-              make_float4(to_f(rc[v].v[0]), to_f(rc[v].v[1]), to_f(rc[v].v[2]), to_f(rc[v].v[3]));
-      }
-    }
-    __syncthreads();
-    if (t0 + kTT < t_hi) fetch(t0 + kTT);
+  Block<MC> A, h;
+  load_A(a, w, c4, n4, A);
+  if (!ENDS && a.nchunk > 1)
+    load_rows<NP>(a.part_h + (((int64_t)w.b * a.nchunk + chunk) * a.Dm + w.d0) * NP, w.nc, c4, n4, h);
+  else
+    load_state(a, w, ENDS ? nullptr : a.h0, c4, n4, h);
+  const bool c0 = pc < w.nc, c1 = pc + 1 < w.nc, whole = a.pair && w.nc == CH;
+  IO* out = (IO*)a.out + (w.b * a.T + t_lo + pr) * a.Dm + w.d0 + pc;
+  const f2 bias = pk(c0 && a.bias ? a.bias[w.d0 + pc] : 0.f, c1 && a.bias ? a.bias[w.d0 + pc + 1] : 0.f);
+  const f2 skip = pk(c0 && a.D ? a.D[w.d0 + pc] : 0.f, c1 && a.D ? a.D[w.d0 + pc + 1] : 0.f);
+  f2 sdt = 0;
+  const int64_t nblk = (a.T + kTT - 1) / kTT;
+  float* hs = a.hsave ? a.hsave + ((w.b * nblk + t_lo / kTT) * a.Dm + w.d0) * NP : nullptr;
 
-#pragma unroll 1
-    for (int tg = 0; tg < kTT; tg += LPC) {
-      if (!ENDS && a.hsave && tg % kSaveSteps == 0 && mine && t0 + tg < a.T) {
-        float* hs = a.hsave + ((b * nblk + (t0 + tg) / kSaveSteps) * a.Dm + d0 + ch) * NP + l * SPT;
+  for (int s = 0; left > 0; left -= kTT, s ^= 1) {
+    const int rows = left;  // of this tile, where below kTT
+    if (left > kTT) {
+      fetch(left - kTT, s ^ 1);
+      cp_wait<1>();
+    } else {
+      cp_wait<0>();
+    }
+    __syncwarp();
+    auto& raw = sm.raw[s];
 #pragma unroll
-        for (int i = 0; i < P2; ++i) reinterpret_cast<float2*>(hs)[i] = up(h[i]);
-      }
-      float p[LPC];
+    for (int k = 0; k < kTT; k += PR) {
+      const int tt = pr + k;
+      f2 x = add2(ld2(&raw.rows[0][tt][pc]), bias);
+      if (a.softplus) x = softplus_2(x);
+      if (tt >= rows) x = 0;
+      if (ENDS) sdt = add2(sdt, x);
+      st2(&sm.dt[tt][pc], x);
+      st2(&sm.du[tt][pc], mul2(x, ld2(&raw.rows[1][tt][pc])));
+    }
+    widen<IO, NP>(sm.b, &raw.bc[0][0][0], lane);
+    if (!ENDS) widen<IO, NP>(sm.c, &raw.bc[SM::kBC - 1][0][0], lane);
+    __syncwarp();
+    if (!ENDS && hs) {
+      store_rows<NP>(hs, w.nc, c4, n4, h);
+      hs += (int64_t)a.Dm * NP;
+    }
+
 #pragma unroll
-      for (int j = 0; j < LPC; ++j) {
-        const int tt = tg + j;
-        if (!ENDS && LPC > kSaveSteps && j == kSaveSteps && a.hsave && mine && t0 + tt < a.T) {
-          float* hs = a.hsave + ((b * nblk + (t0 + tt) / kSaveSteps) * a.Dm + d0 + ch) * NP + l * SPT;
+    for (int ts = 0; ts < kTT; ts += SY) {
+      float p[SY * MC];
 #pragma unroll
-          for (int i = 0; i < P2; ++i) reinterpret_cast<float2*>(hs)[i] = up(h[i]);
-        }
-        const float2 q = s_dt[tt][ch];
-        const f2 dt2 = pk(q.x, q.x), du2 = pk(q.y, q.y);
-        const f2* Bv = reinterpret_cast<const f2*>(&s_b[tt][l * SPT]);
-        const f2* Cv = reinterpret_cast<const f2*>(&s_c[ENDS ? 0 : tt][l * SPT]);
-        f2 acc = 0;
-#pragma unroll
-        for (int i = 0; i < P2; ++i) {
-          h[i] = fma2(ex2_2(mul2(A2[i], dt2)), h[i], mul2(du2, Bv[i]));
-          if (!ENDS) acc = i == 0 ? mul2(Cv[i], h[i]) : fma2(Cv[i], h[i], acc);
-        }
-        if (!ENDS) {
-          const float2 s = up(acc);
-          p[j] = s.x + s.y;
-        }
+      for (int j = 0; j < SY; ++j) {
+        const int tt = ts + j;
+        advance(h, h, A, Chans<MC>(&sm.dt[tt][c4]), Chans<MC>(&sm.du[tt][c4]), States(&sm.b[tt][n4]));
+        if (!ENDS) dot(p + j * MC, h, States(&sm.c[tt][n4]));
       }
       if (!ENDS) {
-        reduce_scatter<LPC, 1>(p, lane);
-        s_y[tg + l][ch] = p[0];
+        reduce_part<SY * MC, LPC, 1>(p, lane);
+        constexpr int R = SY * MC / LPC;  // values a lane keeps: its channels l R .. of step ts + l R / MC
+#pragma unroll
+        for (int r = 0; r < R; ++r) sm.y[ts + l * R / MC][c4 + l * R % MC + r] = p[r];
       }
     }
-    __syncthreads();
+    __syncwarp();
     if (!ENDS) {
 #pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const int tt = rrow + v * RT::kRowStep;
-        if (t0 + tt >= t_hi) continue;
-        const bool live = t0 + tt < len;
-        Vec<IO, W> o;
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          float y = fmaf(Dv[i], to_f(cu[v].v[i]), s_y[tt][rcol + i]);
-          if (zp_) {
-            const float zz = to_f(cz[v].v[i]);
-            y *= zz * sigmoid(zz);
-          }
-          from_f(o.v[i], live ? y : 0.f);
+      for (int k = 0; k < kTT; k += PR) {
+        const int tt = pr + k;
+        f2 y = fma2(skip, ld2(&raw.rows[1][tt][pc]), ld2(&sm.y[tt][pc]));
+        if (Z) {
+          const f2 z = ld2(&raw.rows[SM::kRows - 1][tt][pc]);
+          y = mul2(y, mul2(z, sigmoid_2(z)));
         }
-        store_row<IO, W>((IO*)a.out + (b * a.T + t0 + tt) * a.Dm + d0, rcol, nc, a.vec, o);
+        if (tt < rows) store2(out + k * (int64_t)a.Dm, y, whole, c0, c1);
       }
+      out += kTT * (int64_t)a.Dm;
+      __syncwarp();  // the fetch after next writes these rows
     }
   }
   if (ENDS) {
-    if (mine) {
-      float* ph = a.part_h + (((int64_t)b * a.nchunk + chunk) * a.Dm + d0 + ch) * NP + l * SPT;
+    const int64_t at = ((int64_t)w.b * a.nchunk + chunk) * a.Dm + w.d0;
+    store_rows<NP>(a.part_h + at * NP, w.nc, c4, n4, h);
+    const float2 v = up(over_rows<PC>(sdt));
+    if (pr == 0 && c0) a.part_dt[at + pc] = v.x;
+    if (pr == 0 && c1) a.part_dt[at + pc + 1] = v.y;
+  } else {
+    out = (IO*)a.out + w.b * a.T * a.Dm + w.d0 + pc;
+    for (int64_t t = (t_live > t_lo ? t_live : t_lo) + pr; t < t_hi; t += PR)  // zeros past the length
+      store2(out + t * a.Dm, 0, whole, c0, c1);
+    if (chunk == a.nchunk - 1) store_state(a, w, a.hT, c4, n4, h);
+  }
+}
+
+// The chunks' records in order (BACK: from the last): record c, the end state from zero, becomes the state that enters
+// chunk c. A thread takes 4 states of a channel, its loads kAhead records ahead of the serial chain: as a prologue of
+// every chunk's warps it cost 42 us of 70 at 64 chunks.
+constexpr int kCarryThr = 128, kAhead = 8;
+template <int NP, bool BACK>
+__global__ void __launch_bounds__(kCarryThr) k_sscan_carry(const ScanArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * kCarryThr + threadIdx.x, row = i / (NP / 4);  // b * Dm + d
+  if (row >= (int64_t)a.Bsz * a.Dm) return;
+  const int n4 = (int)(i % (NP / 4)) * 4, b = (int)(row / a.Dm), d = (int)(row % a.Dm);
+  const float* s = BACK ? a.dhT : a.h0;
+  float A[4], h[4];
 #pragma unroll
-      for (int i = 0; i < P2; ++i) reinterpret_cast<float2*>(ph)[i] = up(h[i]);
+  for (int k = 0; k < 4; ++k) {
+    A[k] = n4 + k < a.N ? a.A[(int64_t)d * a.N + n4 + k] * kLog2e : 0.f;
+    h[k] = s && n4 + k < a.N ? s[row * a.N + n4 + k] : 0.f;
+  }
+  // the record that enters last has no end state: chunk nchunk - 1 (BACK: 0)
+  const int64_t step = (BACK ? -1 : 1) * (int64_t)a.Dm, first = (int64_t)b * a.nchunk * a.Dm + d +
+                                                                 (BACK ? (a.nchunk - 1) * (int64_t)a.Dm : 0);
+  for (int c0 = 0; c0 < a.nchunk; c0 += kAhead) {
+    float4 e[kAhead];
+    float dt[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const bool on = c0 + k < a.nchunk - 1;
+      const int64_t at = first + (on ? c0 + k : 0) * step;
+      e[k] = *reinterpret_cast<const float4*>(a.part_h + at * NP + n4);
+      dt[k] = a.part_dt[at];
     }
-    // the chunk's sum of dt per channel, over the threads that share its columns
-    __syncthreads();
-    float* red = reinterpret_cast<float*>(s_dt);  // [kRowStep][CH]
 #pragma unroll
-    for (int i = 0; i < W; ++i) red[rrow * CH + rcol + i] = sdt[i];
-    __syncthreads();
-    if (tid < nc) {
-      float s = 0.f;
-      for (int r = 0; r < RT::kRowStep; ++r) s += red[r * CH + tid];
-      a.part_dt[((int64_t)b * a.nchunk + chunk) * a.Dm + d0 + tid] = s;
-    }
-  } else if (mine && chunk == a.nchunk - 1) {
-#pragma unroll
-    for (int i = 0; i < P2; ++i) {
-      const float2 v = up(h[i]);
-      const int n = l * SPT + 2 * i;
-      float* o = a.hT + ((int64_t)b * a.Dm + d0 + ch) * a.N + n;
-      if (n < a.N) o[0] = v.x;
-      if (n + 1 < a.N) o[1] = v.y;
+    for (int k = 0; k < kAhead; ++k) {
+      if (c0 + k >= a.nchunk) break;
+      *reinterpret_cast<float4*>(a.part_h + (first + (c0 + k) * step) * NP + n4) = make_float4(h[0], h[1], h[2], h[3]);
+      h[0] = fmaf(ex2(A[0] * dt[k]), h[0], e[k].x);
+      h[1] = fmaf(ex2(A[1] * dt[k]), h[1], e[k].y);
+      h[2] = fmaf(ex2(A[2] * dt[k]), h[2], e[k].z);
+      h[3] = fmaf(ex2(A[3] * dt[k]), h[3], e[k].w);
     }
   }
 }
@@ -356,381 +479,353 @@ __global__ void __launch_bounds__(kStepThr) k_sscan_step(const ScanArgs a, int v
 //   dC_t = sum_d dy_t h_t,  dB_t = sum_d g_t dt_t u_t,  s1_t = sum_n g_t B_t,  w = g_t a_t h_{t-1},
 //   du = dt s1 + D dy,  d dt = sum_n w A + u s1,  dA = sum_t w dt,  ddelta = d dt sigmoid(delta + bias),
 //   dz = dout (y + D u) silu'(z),  dD = sum dy u.
-// The forward's state before every 16th step is read back; each block of 16 steps is walked forward once more
-// (a_t and a_t h_{t-1} stay in registers: 2 states a lane) and then backward. Sums over a channel's states
-// are the forward's transposed reductions; sums over channels (dB, dC) go over the warp's
-// channels by shuffles, over the CTA's warps through shared memory, and over CTAs by a buffer of one
-// record per channel tile that k_sscan_dbc adds in a fixed order (no atomics: the same inputs give the same bits).
-constexpr int kBwdThr = 256;
+// The forward's state before every tile is read back; the tile is walked forward once more, its kTT states kept in
+// registers (kTT x kMc x kSpt of them), and then backward, where a_t is computed again: keeping it too would halve the
+// tile. Sums over a channel's states are the forward's transposed reductions; sums over channels (dB, dC) go over
+// the lane's channels in registers, over the warp's by exchanges, over the CTA's warps through shared memory, and
+// over CTAs by a buffer of one record per CTA that k_sscan_dbc adds in a fixed order (no atomics: the same
+// inputs give the same bits).
 
-// Chunk adjoints for a cut time axis: the gradient reaching the state before the chunk's first step from the
-// chunk's own outputs (grid as forward; chunks 1 .. nchunk - 1), and the chunk's sum of dt.
-template <class IO, int NP, int SPT>
-__global__ void __launch_bounds__(kFwdThr) k_sscan_bwd_ends(const ScanArgs a) {
-  constexpr int LPC = NP / SPT, CH = kFwdThr / LPC, P2 = SPT / 2;
-  using RT = RowTile<IO, CH, kFwdThr, kTT>;
-  constexpr int W = RT::W, NV = RT::kVecs;
-  constexpr int BU = kTT * NP / 4 / kFwdThr > 0 ? kTT * NP / 4 / kFwdThr : 1;
-  __shared__ __align__(16) float2 s_dt[kTT][CH];  // dt, dy
-  __shared__ __align__(16) float s_c[kTT][NP];
-  const int tid = threadIdx.x, lane = tid & 31, l = lane % LPC, ch = tid / LPC;
-  const int Dg = a.Dm / a.G, tiles = (Dg + CH - 1) / CH;
-  const int b = blockIdx.x / (tiles * a.G), gt = blockIdx.x - b * tiles * a.G;
-  const int g = gt / tiles, cbase = (gt - g * tiles) * CH;
-  const int chunk = blockIdx.y + 1;
-  const int64_t t_lo = (int64_t)chunk * a.chunk, t_end = t_lo + a.chunk < a.T ? t_lo + a.chunk : a.T;
-  const int64_t len = row_len(a.len, b, a.T), t_hi = t_end < len ? t_end : len;
-  const int nc = Dg - cbase < CH ? Dg - cbase : CH;
-  const int64_t d0 = (int64_t)g * Dg + cbase;
-  const IO* dp_ = (const IO*)a.delta + b * a.d_sb + d0;
-  const IO* zp_ = a.z ? (const IO*)a.z + b * a.z_sb + d0 : nullptr;
-  const IO* op_ = (const IO*)a.dout + b * a.o_sb + d0;
-  const IO* cp_ = (const IO*)a.Cm + b * a.C_sb + g * a.C_sg;
-  const int rcol = (tid % RT::kCols) * W, rrow = tid / RT::kCols;
-  const bool mine = ch < nc;
-  f2 A2[P2], q[P2];
-#pragma unroll
-  for (int i = 0; i < P2; ++i) {
-    const int n = l * SPT + 2 * i;
-    const float* Ap = a.A + (d0 + (mine ? ch : 0)) * a.N;
-    A2[i] = pk(mine && n < a.N ? Ap[n] * kLog2e : 0.f, mine && n + 1 < a.N ? Ap[n + 1] * kLog2e : 0.f);
-    q[i] = 0;
-  }
-  float bias[W], sdt[W];
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
-    bias[i] = rcol + i < nc && a.bias ? a.bias[d0 + rcol + i] : 0.f;
-    sdt[i] = 0.f;
-  }
-  const int64_t ntile = t_hi > t_lo ? (t_hi - t_lo + kTT - 1) / kTT : 0;
-  for (int64_t it = ntile - 1; it >= 0; --it) {
-    const int64_t t0 = t_lo + it * kTT;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int tt = rrow + v * RT::kRowStep;
-      const int64_t t = t0 + tt;
-      const bool live = t < t_hi;
-      Vec<IO, W> rd = zero_row<IO, W>(), ro = rd, rz = rd;
-      if (live) {
-        rd = load_row<IO, W>(dp_ + t * a.d_st, rcol, nc, a.vec);
-        ro = load_row<IO, W>(op_ + t * a.o_st, rcol, nc, a.vec);
-        if (zp_) rz = load_row<IO, W>(zp_ + t * a.z_st, rcol, nc, a.vec);
-      }
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        float x = to_f(rd.v[i]) + bias[i], dy = to_f(ro.v[i]);
-        if (a.softplus) x = softplus(x);
-        if (!live) x = 0.f;
-        if (zp_) dy *= to_f(rz.v[i]) * sigmoid(to_f(rz.v[i]));
-        sdt[i] += x;
-        s_dt[tt][rcol + i] = make_float2(x, dy);
-      }
-    }
-#pragma unroll
-    for (int v = 0; v < BU; ++v) {
-      const int at = tid + v * kFwdThr, tt = at / (NP / 4), n = (at % (NP / 4)) * 4;
-      if (tt < kTT) {
-        Vec<IO, 4> r = zero_row<IO, 4>();
-        if (t0 + tt < t_hi) r = load_row<IO, 4>(cp_ + (t0 + tt) * a.C_st, n, a.N, a.vecbc);
-        *reinterpret_cast<float4*>(&s_c[tt][n]) = make_float4(to_f(r.v[0]), to_f(r.v[1]), to_f(r.v[2]), to_f(r.v[3]));
-      }
-    }
-    __syncthreads();
-#pragma unroll 8
-    for (int tt = kTT - 1; tt >= 0; --tt) {
-      const float2 e = s_dt[tt][ch];
-      const f2 dt2 = pk(e.x, e.x), dy2 = pk(e.y, e.y);
-      const f2* Cv = reinterpret_cast<const f2*>(&s_c[tt][l * SPT]);
-#pragma unroll
-      for (int i = 0; i < P2; ++i) q[i] = mul2(ex2_2(mul2(A2[i], dt2)), fma2(Cv[i], dy2, q[i]));
-    }
-    __syncthreads();
-  }
-  if (mine) {
-    float* ph = a.part_h + (((int64_t)b * a.nchunk + chunk) * a.Dm + d0 + ch) * NP + l * SPT;
-#pragma unroll
-    for (int i = 0; i < P2; ++i) reinterpret_cast<float2*>(ph)[i] = up(q[i]);
-  }
-  __syncthreads();
-  float* red = reinterpret_cast<float*>(s_dt);
-#pragma unroll
-  for (int i = 0; i < W; ++i) red[rrow * CH + rcol + i] = sdt[i];
-  __syncthreads();
-  if (tid < nc) {
-    float s = 0.f;
-    for (int r = 0; r < RT::kRowStep; ++r) s += red[r * CH + tid];
-    a.part_dt[((int64_t)b * a.nchunk + chunk) * a.Dm + d0 + tid] = s;
-  }
-}
-
-template <int NP>
-struct BwdSmem {
-  static constexpr int LPC = NP / 2, CH = kBwdThr / LPC, CPW = 32 / LPC, YS = CH + CPW, WARPS = kBwdThr / 32;
-  static constexpr int q = 0;                                // float4 [kTT][CH]: dt, dt u, dy
-  static constexpr int b = q + kTT * CH * 16, c = b + kTT * NP * 4;
-  static constexpr int y = c + kTT * NP * 4;                 // float [3][kTT][YS]: y, s1, s2
-  static constexpr int red = y + 3 * kTT * YS * 4;           // float [WARPS][kTT][2][NP]: d B, d C of a warp's channels
-  static constexpr int bytes = red + WARPS * kTT * 2 * NP * 4;
+template <class IO, int NP, bool Z>
+struct EndsSmem {  // one warp's
+  static constexpr int CH = Shape<NP, kMcBwd<NP>>::CH;
+  struct Raw {
+    alignas(16) IO rows[Z ? 3 : 2][kTT][CH];  // delta, dout, z
+    alignas(16) IO bc[kTT][NP];
+  };
+  Raw raw[2];
+  alignas(16) float dt[kTT][CH];
+  alignas(16) float dy[kTT][CH];
+  alignas(16) float c[kTT][NP];
 };
 
-template <class IO, int NP>
-__global__ void __launch_bounds__(kBwdThr, 2) k_sscan_bwd(const ScanArgs a) {
-  using SM = BwdSmem<NP>;
-  constexpr int LPC = SM::LPC, CH = SM::CH, CPW = SM::CPW, YS = SM::YS, WARPS = SM::WARPS;
-  constexpr int RG = LPC < 16 ? LPC : 16;          // steps per reduction over a channel's lanes
-  constexpr int CG = CPW >= 2 ? CPW / 2 : 1;       // steps per reduction over the warp's channels
-  using RT = RowTile<IO, CH, kBwdThr, kTT>;
-  constexpr int W = RT::W, NV = RT::kVecs;
-  constexpr int BU = kTT * NP / 4 / kBwdThr > 0 ? kTT * NP / 4 / kBwdThr : 1;
-  extern __shared__ __align__(16) unsigned char sm[];
-  float4(*s_q)[CH] = reinterpret_cast<float4(*)[CH]>(sm + SM::q);
-  float(*s_b)[NP] = reinterpret_cast<float(*)[NP]>(sm + SM::b);
-  float(*s_c)[NP] = reinterpret_cast<float(*)[NP]>(sm + SM::c);
-  float(*s_y)[YS] = reinterpret_cast<float(*)[YS]>(sm + SM::y);
-  float(*s_1)[YS] = s_y + kTT;
-  float(*s_2)[YS] = s_1 + kTT;
-  float* s_red = reinterpret_cast<float*>(sm + SM::red);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l = lane % LPC, cw = lane / LPC, ch = tid / LPC;
-  const int Dg = a.Dm / a.G, tiles = (Dg + CH - 1) / CH;
-  const int b = blockIdx.x / (tiles * a.G), gt = blockIdx.x - b * tiles * a.G;
-  const int g = gt / tiles, cbase = (gt - g * tiles) * CH;
-  const int chunk = blockIdx.y;
+// Chunk adjoints for a cut time axis: the gradient reaching the state before the chunk's first step from the
+// chunk's own outputs (chunks 1 .. nchunk - 1), and the chunk's sum of dt.
+template <class IO, int NP, bool Z>
+__global__ void __launch_bounds__(32 * kWarps) k_sscan_bwd_ends(const ScanArgs a) {
+  using SM = EndsSmem<IO, NP, Z>;
+  constexpr int MC = kMcBwd<NP>;
+  using S = Shape<NP, MC>;
+  constexpr int LPC = S::LPC, CH = S::CH, PC = S::PC, PR = S::PR;
+  extern __shared__ __align__(16) unsigned char sm_raw[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % LPC;
+  SM& sm = reinterpret_cast<SM*>(sm_raw)[warp];
+  const Place<CH> w(a, warp);
+  if (!w.nc) return;
+  const int chunk = blockIdx.y + 1, c4 = lane / LPC * MC, n4 = l * kSpt;
   const int64_t t_lo = (int64_t)chunk * a.chunk, t_end = t_lo + a.chunk < a.T ? t_lo + a.chunk : a.T;
-  const int64_t len = row_len(a.len, b, a.T), t_hi = t_end < len ? t_end : len;  // live steps: t_lo .. t_hi - 1
-  const int nc = Dg - cbase < CH ? Dg - cbase : CH;
-  const int64_t d0 = (int64_t)g * Dg + cbase;
-  const IO* up_ = (const IO*)a.u + b * a.u_sb + d0;
-  const IO* dp_ = (const IO*)a.delta + b * a.d_sb + d0;
-  const IO* zp_ = a.z ? (const IO*)a.z + b * a.z_sb + d0 : nullptr;
-  const IO* op_ = (const IO*)a.dout + b * a.o_sb + d0;
-  const IO* bp_ = (const IO*)a.Bm + b * a.B_sb + g * a.B_sg;
-  const IO* cp_ = (const IO*)a.Cm + b * a.C_sb + g * a.C_sg;
-  const int rcol = (tid % RT::kCols) * W, rrow = tid / RT::kCols;
-  const int64_t nblk = (a.T + kSaveSteps - 1) / kSaveSteps;
-  const bool mine = ch < nc;
-  const int n0 = l * 2;
-
-  f2 A2, q;
-  {
-    const int64_t row = (int64_t)b * a.Dm + d0 + (mine ? ch : 0);
-    const float* Ap = a.A + (d0 + (mine ? ch : 0)) * a.N;
-    const float a0 = mine && n0 < a.N ? Ap[n0] * kLog2e : 0.f, a1 = mine && n0 + 1 < a.N ? Ap[n0 + 1] * kLog2e : 0.f;
-    float q0 = 0.f, q1 = 0.f;
-    if (mine && a.dhT) {
-      if (n0 < a.N) q0 = a.dhT[row * a.N + n0];
-      if (n0 + 1 < a.N) q1 = a.dhT[row * a.N + n0 + 1];
+  const int64_t t_live = t_end < w.len ? t_end : w.len;
+  const int pc = lane % PC * 2, pr = lane / PC;
+  const int ntile = t_live > t_lo ? (int)((t_live - t_lo + kTT - 1) / kTT) : 0;
+  const int64_t t_at = t_lo + (ntile ? ntile - 1 : 0) * (int64_t)kTT;  // the last tile comes first
+  using Rows = Feed<IO, kTT, CH>;
+  Rows fd((const IO*)a.delta + w.b * a.d_sb + t_at * a.d_st + w.d0, a.d_st, w.nc, a.vec, lane);
+  Rows fo((const IO*)a.dout + w.b * a.o_sb + t_at * a.o_st + w.d0, a.o_st, w.nc, a.vec, lane);
+  Rows fz(Z ? (const IO*)a.z + w.b * a.z_sb + t_at * a.z_st + w.d0 : nullptr, a.z_st, w.nc, a.vec, lane);
+  Feed<IO, kTT, NP> fc((const IO*)a.Cm + w.b * a.C_sb + w.g * a.C_sg + t_at * a.C_st, a.C_st, a.N, a.vecbc, lane);
+  auto fetch = [&](int rows, int s) {
+    auto& r = sm.raw[s];
+    fd.tile(&r.rows[0][0][0], a.d_st, rows, a.vec, lane);
+    fo.tile(&r.rows[1][0][0], a.o_st, rows, a.vec, lane);
+    fd.p -= kTT * a.d_st, fo.p -= kTT * a.o_st;
+    if (Z) {
+      fz.tile(&r.rows[Z ? 2 : 0][0][0], a.z_st, rows, a.vec, lane);
+      fz.p -= kTT * a.z_st;
     }
-    if (mine)
-      for (int c = a.nchunk - 1; c > chunk; --c) {
-        const int64_t at = ((int64_t)b * a.nchunk + c) * a.Dm + d0 + ch;
-        const float sdt = a.part_dt[at];
-        const float2 p = *reinterpret_cast<const float2*>(a.part_h + at * NP + n0);
-        q0 = fmaf(ex2(a0 * sdt), q0, p.x);
-        q1 = fmaf(ex2(a1 * sdt), q1, p.y);
-      }
-    A2 = pk(a0, a1);
-    q = pk(q0, q1);
-  }
-  float bias[W], Dv[W], accD[W], accb[W];
+    fc.tile(&r.bc[0][0], a.C_st, rows, a.vecbc, lane);
+    fc.p -= kTT * a.C_st;
+    cp_commit();
+  };
+  if (ntile) fetch((int)(t_live - t_at), 0);
+  Block<MC> A, q;
+  load_A(a, w, c4, n4, A);
+  load_state(a, w, nullptr, c4, n4, q);
+  const bool c0 = pc < w.nc, c1 = pc + 1 < w.nc;
+  const f2 bias = pk(c0 && a.bias ? a.bias[w.d0 + pc] : 0.f, c1 && a.bias ? a.bias[w.d0 + pc + 1] : 0.f);
+  f2 sdt = 0;
+  int rows = (int)(t_live - t_at);
+  for (int it = ntile - 1, s = 0; it >= 0; --it, s ^= 1, rows = kTT) {
+    if (it > 0) {
+      fetch(kTT, s ^ 1);
+      cp_wait<1>();
+    } else {
+      cp_wait<0>();
+    }
+    __syncwarp();
+    auto& raw = sm.raw[s];
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    const bool ok = rcol + i < nc;
-    bias[i] = ok && a.bias ? a.bias[d0 + rcol + i] : 0.f;
-    Dv[i] = ok && a.D ? a.D[d0 + rcol + i] : 0.f;
-    accD[i] = accb[i] = 0.f;
+    for (int k = 0; k < kTT; k += PR) {
+      const int tt = pr + k;
+      f2 x = add2(ld2(&raw.rows[0][tt][pc]), bias), dy = ld2(&raw.rows[1][tt][pc]);
+      if (a.softplus) x = softplus_2(x);
+      if (tt >= rows) x = 0;
+      if (Z) {
+        const f2 z = ld2(&raw.rows[Z ? 2 : 0][tt][pc]);
+        dy = mul2(dy, mul2(z, sigmoid_2(z)));
+      }
+      sdt = add2(sdt, x);
+      st2(&sm.dt[tt][pc], x);
+      st2(&sm.dy[tt][pc], dy);
+    }
+    widen<IO, NP>(sm.c, &raw.bc[0][0], lane);
+    __syncwarp();
+#pragma unroll
+    for (int tt = kTT - 1; tt >= 0; --tt) {
+      const Chans<MC> dt(&sm.dt[tt][c4]), dy(&sm.dy[tt][c4]);
+      const States C(&sm.c[tt][n4]);
+#pragma unroll
+      for (int c = 0; c < MC; ++c)
+#pragma unroll
+        for (int p = 0; p < kSpt / 2; ++p)
+          q.v[c][p] = mul2(ex2_2(mul2(A.v[c][p], dt.v[c])), fma2(C.v[p], dy.v[c], q.v[c][p]));
+    }
+    __syncwarp();
   }
-  f2 dA = 0;
+  const int64_t at = ((int64_t)w.b * a.nchunk + chunk) * a.Dm + w.d0;
+  store_rows<NP>(a.part_h + at * NP, w.nc, c4, n4, q);
+  const float2 v = up(over_rows<PC>(sdt));
+  if (pr == 0 && c0) a.part_dt[at + pc] = v.x;
+  if (pr == 0 && c1) a.part_dt[at + pc + 1] = v.y;
+}
+
+template <class IO, int NP, bool Z>
+struct BwdSmem {
+  static constexpr int CH = Shape<NP, kMcBwd<NP>>::CH;
+  struct Raw {
+    alignas(16) IO rows[Z ? 4 : 3][kTT][CH];  // delta, u, dout, z
+    alignas(16) float h[CH][NP];      // the state before the tile
+  };
+  struct Warp {
+    Raw raw[2];
+    alignas(16) IO bc[2][kTT][NP];
+    alignas(16) float dt[kTT][CH];
+    alignas(16) float du[kTT][CH];
+    alignas(16) float dy[kTT][CH];
+    alignas(16) float b[kTT][NP];
+    alignas(16) float c[kTT][NP];
+    alignas(16) float y[Z ? 3 : 2][kTT][CH];  // s1, s2, y
+  };
+  Warp warp[kWarps];
+  alignas(16) float red[2][kWarps][kTT][2][NP];  // d B, d C over a warp's channels, two tiles' worth
+};
+
+template <class IO, int NP, bool Z>
+__global__ void __launch_bounds__(32 * kWarps, kBwdCtas) k_sscan_bwd(const ScanArgs a) {
+  using SM = BwdSmem<IO, NP, Z>;
+  constexpr int MC = kMcBwd<NP>;
+  using S = Shape<NP, MC>;
+  constexpr int LPC = S::LPC, CH = S::CH, PC = S::PC, PR = S::PR, SY = S::SY, SB = S::SB, Q = S::Q;
+  extern __shared__ __align__(16) unsigned char sm_raw[];
+  SM& all = *reinterpret_cast<SM*>(sm_raw);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % LPC, qd = lane / LPC;
+  auto& sm = all.warp[warp];
+  const Place<CH> w(a, warp);  // a warp without channels walks along with zeros: the CTA adds over its warps
+  const int chunk = blockIdx.y, c4 = qd * MC, n4 = l * kSpt;
+  const int64_t t_lo = (int64_t)chunk * a.chunk, t_end = t_lo + a.chunk < a.T ? t_lo + a.chunk : a.T;
+  const int64_t t_live = t_end < w.len ? t_end : w.len;
+  const int64_t nblk = (a.T + kTT - 1) / kTT;
+  const int pc = lane % PC * 2, pr = lane / PC;
+  const int ntile = t_live > t_lo ? (int)((t_live - t_lo + kTT - 1) / kTT) : 0;
+  const int64_t t_at = t_lo + (ntile ? ntile - 1 : 0) * (int64_t)kTT;  // the last tile comes first
+  using Rows = Feed<IO, kTT, CH>;
+  using Cols = Feed<IO, kTT, NP>;
+  Rows fd((const IO*)a.delta + w.b * a.d_sb + t_at * a.d_st + w.d0, a.d_st, w.nc, a.vec, lane);
+  Rows fu((const IO*)a.u + w.b * a.u_sb + t_at * a.u_st + w.d0, a.u_st, w.nc, a.vec, lane);
+  Rows fo((const IO*)a.dout + w.b * a.o_sb + t_at * a.o_st + w.d0, a.o_st, w.nc, a.vec, lane);
+  Rows fz(Z ? (const IO*)a.z + w.b * a.z_sb + t_at * a.z_st + w.d0 : nullptr, a.z_st, w.nc, a.vec, lane);
+  Cols fb((const IO*)a.Bm + w.b * a.B_sb + w.g * a.B_sg + t_at * a.B_st, a.B_st, a.N, a.vecbc, lane);
+  Cols fc((const IO*)a.Cm + w.b * a.C_sb + w.g * a.C_sg + t_at * a.C_st, a.C_st, a.N, a.vecbc, lane);
+  Feed<float, CH, NP> fh(a.hsave + ((w.b * nblk + t_at / kTT) * a.Dm + w.d0) * NP, NP, NP, 1, lane);
+  auto fetch = [&](int rows, int s) {
+    auto& r = sm.raw[s];
+    fd.tile(&r.rows[0][0][0], a.d_st, rows, a.vec, lane);
+    fu.tile(&r.rows[1][0][0], a.u_st, rows, a.vec, lane);
+    fo.tile(&r.rows[2][0][0], a.o_st, rows, a.vec, lane);
+    fd.p -= kTT * a.d_st, fu.p -= kTT * a.u_st, fo.p -= kTT * a.o_st;
+    if (Z) {
+      fz.tile(&r.rows[Z ? 3 : 0][0][0], a.z_st, rows, a.vec, lane);
+      fz.p -= kTT * a.z_st;
+    }
+    fb.tile(&sm.bc[0][0][0], a.B_st, rows, a.vecbc, lane);
+    fc.tile(&sm.bc[1][0][0], a.C_st, rows, a.vecbc, lane);
+    fb.p -= kTT * a.B_st, fc.p -= kTT * a.C_st;
+    fh.tile(&r.h[0][0], NP, w.nc, 1, lane);
+    fh.p -= (int64_t)a.Dm * NP;
+    cp_commit();
+  };
+  if (ntile) fetch((int)(t_live - t_at), 0);
+
+  Block<MC> A, q, dA;
+  load_A(a, w, c4, n4, A);
+  if (a.nchunk > 1)
+    load_rows<NP>(a.part_h + (((int64_t)w.b * a.nchunk + chunk) * a.Dm + w.d0) * NP, w.nc, c4, n4, q);
+  else
+    load_state(a, w, a.dhT, c4, n4, q);
+  load_state(a, w, nullptr, c4, n4, dA);
+  const bool c0 = pc < w.nc, c1 = pc + 1 < w.nc, whole = a.pair && w.nc == CH;
+  const f2 bias = pk(c0 && a.bias ? a.bias[w.d0 + pc] : 0.f, c1 && a.bias ? a.bias[w.d0 + pc + 1] : 0.f);
+  const f2 skip = pk(c0 && a.D ? a.D[w.d0 + pc] : 0.f, c1 && a.D ? a.D[w.d0 + pc + 1] : 0.f);
+  f2 accD = 0, accb = 0;
+  float* dbc = a.dbc + ((int64_t)w.tile * a.Bsz + w.b) * a.T * 2 * NP;
 
   // rows past the length: zero gradients
-  const int64_t dead = t_lo > len ? t_lo : len;
-  for (int64_t i = tid; i < (t_end - dead) * nc; i += kBwdThr) {
-    const int64_t at = (b * a.T + dead + i / nc) * a.Dm + d0 + i % nc;
-    from_f(((IO*)a.du)[at], 0.f);
-    from_f(((IO*)a.ddelta)[at], 0.f);
-    if (a.dz) from_f(((IO*)a.dz)[at], 0.f);
+  const int64_t dead = t_lo > w.len ? t_lo : w.len;
+  for (int64_t t = dead + pr; t < t_end; t += PR) {
+    const int64_t at = (w.b * a.T + t) * a.Dm + w.d0 + pc;
+    store2((IO*)a.du + at, 0, whole, c0, c1);
+    store2((IO*)a.ddelta + at, 0, whole, c0, c1);
+    if (Z) store2((IO*)a.dz + at, 0, whole, c0, c1);
   }
-  if (a.dbc)
-    for (int64_t i = tid; i < (t_end - dead) * 2 * NP; i += kBwdThr)
-      a.dbc[(((int64_t)gt * a.Bsz + b) * a.T + dead) * 2 * NP + i] = 0.f;
+  for (int64_t i = threadIdx.x; i < (t_end - dead) * 2 * NP; i += 32 * kWarps) dbc[dead * 2 * NP + i] = 0.f;
 
-  const int64_t ntile = t_hi > t_lo ? (t_hi - t_lo + kTT - 1) / kTT : 0;
-  for (int64_t it = ntile - 1; it >= 0; --it) {
-    const int64_t t0 = t_lo + it * kTT;
-    Vec<IO, W> ru[NV], rd[NV], rz[NV], ro[NV];
+  int64_t at = (w.b * a.T + t_at + pr) * a.Dm + w.d0 + pc;  // the lane's place in the row outputs
+  dbc += t_at * 2 * NP;
+  int rows = (int)(t_live - t_at);
+  for (int it = ntile - 1, s = 0; it >= 0; --it, s ^= 1, rows = kTT) {
+    cp_wait<0>();
+    __syncwarp();
+    auto& raw = sm.raw[s];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int tt = rrow + v * RT::kRowStep;
-      const int64_t t = t0 + tt;
-      const bool live = t < t_hi;
-      ru[v] = rd[v] = rz[v] = ro[v] = zero_row<IO, W>();
-      if (live) {
-        ru[v] = load_row<IO, W>(up_ + t * a.u_st, rcol, nc, a.vec);
-        rd[v] = load_row<IO, W>(dp_ + t * a.d_st, rcol, nc, a.vec);
-        ro[v] = load_row<IO, W>(op_ + t * a.o_st, rcol, nc, a.vec);
-        if (zp_) rz[v] = load_row<IO, W>(zp_ + t * a.z_st, rcol, nc, a.vec);
+    for (int k = 0; k < kTT; k += PR) {
+      const int tt = pr + k;
+      f2 x = add2(ld2(&raw.rows[0][tt][pc]), bias), dy = ld2(&raw.rows[2][tt][pc]);
+      if (a.softplus) x = softplus_2(x);
+      if (tt >= rows) x = 0;
+      if (Z) {
+        const f2 z = ld2(&raw.rows[Z ? 3 : 0][tt][pc]);
+        dy = mul2(dy, mul2(z, sigmoid_2(z)));
       }
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        float x = to_f(rd[v].v[i]) + bias[i], dy = to_f(ro[v].v[i]);
-        if (a.softplus) x = softplus(x);
-        if (!live) x = 0.f;
-        if (zp_) dy *= to_f(rz[v].v[i]) * sigmoid(to_f(rz[v].v[i]));
-        s_q[tt][rcol + i] = make_float4(x, x * to_f(ru[v].v[i]), dy, 0.f);
-      }
+      st2(&sm.dt[tt][pc], x);
+      st2(&sm.du[tt][pc], mul2(x, ld2(&raw.rows[1][tt][pc])));
+      st2(&sm.dy[tt][pc], dy);
     }
-#pragma unroll
-    for (int v = 0; v < BU; ++v) {
-      const int at = tid + v * kBwdThr, tt = at / (NP / 4), n = (at % (NP / 4)) * 4;
-      if (tt < kTT) {
-        Vec<IO, 4> r = zero_row<IO, 4>(), s = r;
-        if (t0 + tt < t_hi) {
-          r = load_row<IO, 4>(bp_ + (t0 + tt) * a.B_st, n, a.N, a.vecbc);
-          s = load_row<IO, 4>(cp_ + (t0 + tt) * a.C_st, n, a.N, a.vecbc);
-        }
-        *reinterpret_cast<float4*>(&s_b[tt][n]) = make_float4(to_f(r.v[0]), to_f(r.v[1]), to_f(r.v[2]), to_f(r.v[3]));
-        *reinterpret_cast<float4*>(&s_c[tt][n]) = make_float4(to_f(s.v[0]), to_f(s.v[1]), to_f(s.v[2]), to_f(s.v[3]));
-      }
-    }
-    __syncthreads();
+    widen<IO, NP>(sm.b, &sm.bc[0][0][0], lane);
+    widen<IO, NP>(sm.c, &sm.bc[1][0][0], lane);
+    __syncwarp();
+    if (it > 0) fetch(kTT, s ^ 1);  // B and C have been taken out of their single buffer
 
-    // d B (part 0) and d C (part 1) of step tt over the warp's channels
-    auto put = [&](float* v, int tt, int part) {  // v: CG steps x 2 states, ending at step tt + CG - 1
-      if (CPW >= 2) {
-        reduce_scatter<CPW >= 2 ? CPW : 2, LPC>(v, lane);
-        s_red[((warp * kTT + tt + cw / 2) * 2 + part) * NP + n0 + (cw & 1)] = v[0];
-      } else {
-        s_red[((warp * kTT + tt) * 2 + part) * NP + n0] = v[0];
-        s_red[((warp * kTT + tt) * 2 + part) * NP + n0 + 1] = v[1];
-      }
+    // sums over a channel's lanes of SY steps from ts, to rows of y
+    auto put_row = [&](float* p, int ts, float (*dst)[CH]) {
+      reduce_part<SY * MC, LPC, 1>(p, lane);
+      constexpr int R = SY * MC / LPC;
+#pragma unroll
+      for (int r = 0; r < R; ++r) dst[ts + l * R / MC][c4 + l * R % MC + r] = p[r];
     };
-    auto put_row = [&](float* v, int tt, float (*dst)[YS]) {  // RG steps from tt
-      reduce_scatter<RG, 1>(v, lane);
-      float r = v[0];
-      if (LPC > RG) r += __shfl_xor_sync(0xffffffffu, r, 16);
-      if (l < RG) dst[tt + l][ch] = r;
+    // sums over the warp's channel groups of SB steps from ts: d B (part 0), d C (part 1)
+    auto put_bc = [&](f2* p, int ts, int part) {
+      reduce_pairs<SB * kSpt / 2, Q, LPC>(p, lane);
+      constexpr int R = SB * kSpt / Q;
+      float* o = &all.red[s][warp][ts + qd * R / kSpt][part][n4 + qd * R % kSpt];
+      if (R == 1) o[0] = up(p[0]).x;
+      else st2(o, p[0]);
+      static_assert(R <= 2, "one pair at most");
     };
 
-#pragma unroll 1
-    for (int blk = kTT / kSaveSteps - 1; blk >= 0; --blk) {
-      const int tb = blk * kSaveSteps;
-      f2 aa[kSaveSteps], ah[kSaveSteps];
-      f2 h = 0;
-      if (mine && t0 + tb < t_hi) {
-        const float2 v = *reinterpret_cast<const float2*>(
-            a.hsave + ((b * nblk + (t0 + tb) / kSaveSteps) * a.Dm + d0 + ch) * NP + n0);
-        h = pk(v.x, v.y);
-      }
-      {
-        float py[RG], pc[2 * CG];
+    Block<MC> hb[kTT];  // the state before each step
+    load_rows<NP>(&raw.h[0][0], CH, c4, n4, hb[0]);
+    {
+      float py[SY * MC];
+      f2 pb[SB * kSpt / 2];
 #pragma unroll
-        for (int j = 0; j < kSaveSteps; ++j) {
-          const float4 e = s_q[tb + j][ch];
-          const f2 Bv = *reinterpret_cast<const f2*>(&s_b[tb + j][n0]);
-          aa[j] = ex2_2(mul2(A2, pk(e.x, e.x)));
-          ah[j] = mul2(aa[j], h);
-          h = fma2(pk(e.y, e.y), Bv, ah[j]);
-          if (zp_) {
-            const float2 y = up(mul2(*reinterpret_cast<const f2*>(&s_c[tb + j][n0]), h));
-            py[j % RG] = y.x + y.y;
-            if (j % RG == RG - 1) put_row(py, tb + j + 1 - RG, s_y);
+      for (int tt = 0; tt < kTT; ++tt) {
+        Block<MC> h;
+        advance(h, hb[tt], A, Chans<MC>(&sm.dt[tt][c4]), Chans<MC>(&sm.du[tt][c4]), States(&sm.b[tt][n4]));
+        if (tt + 1 < kTT) hb[tt + 1 < kTT ? tt + 1 : 0] = h;
+        if (Z) {
+          dot(py + tt % SY * MC, h, States(&sm.c[tt][n4]));
+          if (tt % SY == SY - 1) put_row(py, tt + 1 - SY, sm.y[Z ? 2 : 0]);
+        }
+        const Chans<MC> dy(&sm.dy[tt][c4]);
+#pragma unroll
+        for (int p = 0; p < kSpt / 2; ++p) {
+          f2 v = mul2(dy.v[0], h.v[0][p]);
+#pragma unroll
+          for (int c = 1; c < MC; ++c) v = fma2(dy.v[c], h.v[c][p], v);
+          pb[tt % SB * (kSpt / 2) + p] = v;
+        }
+        if (tt % SB == SB - 1) put_bc(pb, tt + 1 - SB, 1);
+      }
+    }
+    {
+      float p1[SY * MC], p2[SY * MC];
+      f2 pb[SB * kSpt / 2];
+#pragma unroll
+      for (int tt = kTT - 1; tt >= 0; --tt) {
+        const Chans<MC> dt(&sm.dt[tt][c4]), du(&sm.du[tt][c4]), dy(&sm.dy[tt][c4]);
+        const States B(&sm.b[tt][n4]), C(&sm.c[tt][n4]);
+#pragma unroll
+        for (int c = 0; c < MC; ++c) {
+          f2 x1, x2;
+#pragma unroll
+          for (int p = 0; p < kSpt / 2; ++p) {
+            const f2 gg = fma2(C.v[p], dy.v[c], q.v[c][p]);
+            q.v[c][p] = mul2(ex2_2(mul2(A.v[c][p], dt.v[c])), gg);
+            const f2 wv = mul2(q.v[c][p], hb[tt].v[c][p]);  // g a h_{t-1}
+            x1 = p ? fma2(gg, B.v[p], x1) : mul2(gg, B.v[p]);
+            x2 = p ? fma2(wv, A.v[c][p], x2) : mul2(wv, A.v[c][p]);  // in units of log2(e)
+            dA.v[c][p] = fma2(wv, dt.v[c], dA.v[c][p]);
+            f2& vb = pb[tt % SB * (kSpt / 2) + p];
+            vb = c ? fma2(gg, du.v[c], vb) : mul2(gg, du.v[c]);
           }
-          if (a.dbc) {
-            const float2 c = up(mul2(pk(e.z, e.z), h));
-            pc[j % CG * 2] = c.x, pc[j % CG * 2 + 1] = c.y;
-            if (j % CG == CG - 1) put(pc, tb + j + 1 - CG, 1);
-          }
+          const float2 v1 = up(x1), v2 = up(x2);
+          p1[tt % SY * MC + c] = v1.x + v1.y;
+          p2[tt % SY * MC + c] = v2.x + v2.y;
         }
-      }
-      float p1[RG], p2[RG], pb[2 * CG];
-#pragma unroll
-      for (int j = kSaveSteps - 1; j >= 0; --j) {
-        const float4 e = s_q[tb + j][ch];
-        const f2 Bv = *reinterpret_cast<const f2*>(&s_b[tb + j][n0]);
-        const f2 Cv = *reinterpret_cast<const f2*>(&s_c[tb + j][n0]);
-        const f2 gg = fma2(Cv, pk(e.z, e.z), q);
-        const f2 w = mul2(gg, ah[j]);
-        const float2 x1 = up(mul2(gg, Bv)), x2 = up(mul2(w, A2));
-        p1[j % RG] = x1.x + x1.y;
-        p2[j % RG] = x2.x + x2.y;  // in units of A log2(e)
-        dA = fma2(w, pk(e.x, e.x), dA);
-        if (a.dbc) {
-          const float2 c = up(mul2(gg, pk(e.y, e.y)));
-          pb[j % CG * 2] = c.x, pb[j % CG * 2 + 1] = c.y;
-          if (j % CG == 0) put(pb, tb + j, 0);
+        if (tt % SY == 0) {
+          put_row(p1, tt, sm.y[0]);
+          put_row(p2, tt, sm.y[1]);
         }
-        q = mul2(gg, aa[j]);
-        if (j % RG == 0) {
-          put_row(p1, tb + j, s_1);
-          put_row(p2, tb + j, s_2);
-        }
+        if (tt % SB == 0) put_bc(pb, tt, 0);
       }
     }
-    __syncthreads();
+    __syncwarp();
 
-    // the tile's rows: du, ddelta, dz; its share of d D and d bias
+    // the tile's rows: du, ddelta, dz; their share of d D and d bias
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int tt = rrow + v * RT::kRowStep;
-      if (t0 + tt >= t_hi) continue;
-      Vec<IO, W> o1, o2, o3;
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const float4 e = s_q[tt][rcol + i];
-        const float uu = to_f(ru[v].v[i]), s1 = s_1[tt][rcol + i];
-        float dx = fmaf(uu, s1, s_2[tt][rcol + i] * 0.6931471805599453f);
-        if (a.softplus) dx *= sigmoid(to_f(rd[v].v[i]) + bias[i]);
-        from_f(o1.v[i], fmaf(e.x, s1, Dv[i] * e.z));
-        from_f(o2.v[i], dx);
-        if (zp_) {
-          const float zz = to_f(rz[v].v[i]), sg = sigmoid(zz), y = fmaf(Dv[i], uu, s_y[tt][rcol + i]);
-          from_f(o3.v[i], to_f(ro[v].v[i]) * y * sg * fmaf(zz, 1.f - sg, 1.f));
-        }
-        accD[i] = fmaf(e.z, uu, accD[i]);
-        accb[i] += dx;
+    for (int k = 0; k < kTT; k += PR) {
+      const int tt = pr + k;
+      const f2 u = ld2(&raw.rows[1][tt][pc]), dy = ld2(&sm.dy[tt][pc]), s1 = ld2(&sm.y[0][tt][pc]);
+      const f2 du = fma2(ld2(&sm.dt[tt][pc]), s1, mul2(skip, dy));
+      f2 dd = fma2(u, s1, mul2(ld2(&sm.y[1][tt][pc]), both(0.6931471805599453f)));
+      if (a.softplus) dd = mul2(dd, sigmoid_2(add2(ld2(&raw.rows[0][tt][pc]), bias)));
+      const int64_t o = at + k * (int64_t)a.Dm;
+      if (tt < rows) {
+        store2((IO*)a.du + o, du, whole, c0, c1);
+        store2((IO*)a.ddelta + o, dd, whole, c0, c1);
+        accD = fma2(dy, u, accD);
+        accb = add2(accb, dd);
       }
-      const int64_t at = (b * a.T + t0 + tt) * a.Dm + d0;
-      store_row<IO, W>((IO*)a.du + at, rcol, nc, a.vec, o1);
-      store_row<IO, W>((IO*)a.ddelta + at, rcol, nc, a.vec, o2);
-      if (zp_) store_row<IO, W>((IO*)a.dz + at, rcol, nc, a.vec, o3);
-    }
-    if (a.dbc) {
-      const int64_t base = (((int64_t)gt * a.Bsz + b) * a.T + t0) * 2 * NP;
-      for (int i = tid; i < kTT * 2 * NP; i += kBwdThr) {
-        if (t0 + i / (2 * NP) >= t_hi) break;
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) s += s_red[w * kTT * 2 * NP + i];
-        a.dbc[base + i] = s;
+      if (Z) {
+        const f2 z = ld2(&raw.rows[Z ? 3 : 0][tt][pc]), sg = sigmoid_2(z);
+        const f2 y = fma2(skip, u, ld2(&sm.y[Z ? 2 : 0][tt][pc]));
+        // silu'(z) = sg (1 + z (1 - sg))
+        const f2 sl = mul2(sg, fma2(z, fma2(sg, both(-1.f), both(1.f)), both(1.f)));
+        if (tt < rows) store2((IO*)a.dz + o, mul2(mul2(ld2(&raw.rows[2][tt][pc]), y), sl), whole, c0, c1);
       }
     }
+    at -= kTT * (int64_t)a.Dm;
+    __syncthreads();  // one a tile: the records of the other buffer are written next
+#pragma unroll
+    for (int k = 0; k < kTT * 2 * NP / 2; k += 32 * kWarps) {
+      const int i = (k + threadIdx.x) * 2;
+      if (i < (rows < kTT ? rows : kTT) * 2 * NP) {
+        f2 v = 0;
+#pragma unroll
+        for (int j = 0; j < kWarps; ++j) v = add2(v, ld2(&all.red[s][j][0][0][0] + i));
+        st2(dbc + i, v);
+      }
+    }
+    dbc -= kTT * 2 * NP;
   }
 
-  const int64_t part = (int64_t)b * a.nchunk + chunk;
-  if (mine) {
-    *reinterpret_cast<float2*>(a.part_dA + (part * a.Dm + d0 + ch) * NP + n0) = up(dA);
-    if (chunk == 0 && a.dh0) {
-      const float2 v = up(q);
-      float* o = a.dh0 + ((int64_t)b * a.Dm + d0 + ch) * a.N + n0;
-      if (n0 < a.N) o[0] = v.x;
-      if (n0 + 1 < a.N) o[1] = v.y;
-    }
-  }
-  // d D, d bias over the threads that share a column
-  float* red = reinterpret_cast<float*>(s_q);  // [2][kRowStep][CH]
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
-    red[rrow * CH + rcol + i] = accD[i];
-    red[(RT::kRowStep + rrow) * CH + rcol + i] = accb[i];
-  }
-  __syncthreads();
-  if (tid < 2 * CH) {
-    const int which = tid / CH, c = tid % CH;
-    if (c < nc) {
-      float s = 0.f;
-      for (int r = 0; r < RT::kRowStep; ++r) s += red[(which * RT::kRowStep + r) * CH + c];
-      a.part_dD[(part * 2 + which) * a.Dm + d0 + c] = s;
-    }
+  const int64_t part = (int64_t)w.b * a.nchunk + chunk;
+  store_rows<NP>(a.part_dA + (part * a.Dm + w.d0) * NP, w.nc, c4, n4, dA);
+  if (chunk == 0 && a.dh0) store_state(a, w, a.dh0, c4, n4, q);
+  const float2 vD = up(over_rows<PC>(accD)), vb = up(over_rows<PC>(accb));
+  if (pr == 0) {
+    float* o = a.part_dD + part * 2 * a.Dm + w.d0 + pc;
+    if (c0) o[0] = vD.x, o[a.Dm] = vb.x;
+    if (c1) o[1] = vD.y, o[a.Dm + 1] = vb.y;
   }
 }
 
