@@ -286,7 +286,7 @@ const char* const kKernelNames[KID_COUNT] = {
   "k_bwd_grads", "k_bwd_bufout", "k_bwd_finalize", "k_bwd_dsref", "k_fmap_tensor_bwd", "k_fwd_chunk_tc", "k_fwd_out_tc", "k_fwd_buf_y",
   "k_bwd_chunk_tc", "k_bwd_state_gates_tc", "k_bwd_buf_tc", "k_bwd_finalize_tc", "k_bwd_dsref_tc", "k_bwd_keys_tc", "k_sref_tile", "k_decode_step", "k_scan_op_fwd", "k_scan_op_bwd", "k_compose_carries", "k_dwconv3_fwd", "k_dwconv3_bwd", "k_head_prep_fwd", "k_head_prep_bwd", "k_proj_tiles", "k_fmap_fwd_tc", "k_fmap_bwd_tc", "k_omega_store_fwd", "k_omega_store_bwd", "k_affine_scan_fwd", "k_affine_scan_bwd",
   "k_sscan_fwd", "k_sscan_ends", "k_sscan_carry", "k_sscan_step", "k_sscan_bwd", "k_sscan_bwd_ends", "k_sscan_dbc", "k_sscan_dA",
-  "k_causal_conv_fwd", "k_causal_conv_bwd", "k_causal_conv_dw", "k_sample", "k_distill_fwd", "k_distill_bwd"};
+  "k_causal_conv_fwd", "k_causal_conv_step", "k_causal_conv_bwd", "k_causal_conv_dw", "k_sample", "k_distill_fwd", "k_distill_bwd"};
 
 constexpr int kMaxTimed = 8192;
 struct Prof {

@@ -33,6 +33,11 @@ int launch(bool fwd, ConvArgs a, int64_t B, float* dw, float* dbias, cudaStream_
           wide(a.d_final, a.C, a.C, size, W) && wide(a.y, a.C, a.C, size, W) && wide(a.final_state, a.C, a.C, size, W) &&
           wide(a.dx, a.C, a.C, size, W) && wide(a.d_init, a.C, a.C, size, W);
   const dim3 grid((unsigned)(B * a.ygrid), (unsigned)((a.C + 32 * W - 1) / (32 * W)));
+  if (fwd && a.T == 1 && B <= 65535) {
+    const dim3 one((unsigned)((a.C + kConvStepThr * W - 1) / (kConvStepThr * W)), (unsigned)B);
+    LAUNCH_T(KID_CONV_STEP, (k_causal_conv_step<K, IO, W>), one, kConvStepThr, 0, st, a);
+    return ATLAS_OK;
+  }
   if (fwd) {
     LAUNCH_T(KID_CONV_FWD, (k_causal_conv_fwd<K, IO, W>), grid, 32 * kConvWarps, 0, st, a);
     return ATLAS_OK;

@@ -14,17 +14,24 @@
 namespace atlas {
 namespace cc {
 
+using ss::add2;
+using ss::both;
+using ss::ex2_2;
+using ss::f2;
+using ss::fma2;
 using ss::from_f;
-using ss::load_row;
+using ss::ld2;
+using ss::mul2;
+using ss::pk;
 using ss::row_len;
-using ss::sigmoid;
-using ss::store_row;
+using ss::sigmoid_2;
+using ss::st2;
 using ss::to_f;
+using ss::up;
 using ss::Vec;
-using ss::zero_row;
 
 constexpr int kConvWarps = 4;  // runs per CTA
-constexpr int kConvU = 8;      // steps loaded ahead
+constexpr int kConvU = 8;      // steps in flight
 
 struct ConvArgs {
   const void *x, *init, *dy, *d_final;
@@ -37,171 +44,272 @@ struct ConvArgs {
   int run, ygrid, silu, vec;  // steps per thread; CTAs along the time axis
 };
 
-// step t of the row (t >= -(K-1)), the state where t < 0
-template <int K, class IO, int W>
-__device__ __forceinline__ Vec<IO, W> step_row(const ConvArgs& a, const IO* x, const IO* init, int64_t t, int64_t c,
-                                               int nc) {
-  if (t >= 0) return load_row<IO, W>(x + t * a.x_st + c, 0, nc, a.vec);
-  if (init) return load_row<IO, W>(init + (t + K - 1) * a.C + c, 0, nc, a.vec);
-  return zero_row<IO, W>();
+// W channels of a row as pairs: whole vectors where `fast`, else those below nc one by one.
+template <class IO, int W>
+struct Row {
+  f2 v[W / 2];
+};
+template <class IO, int W>
+__device__ __forceinline__ Row<IO, W> widen(const Vec<IO, W>& r) {
+  Row<IO, W> o;
+#pragma unroll
+  for (int i = 0; i < W / 2; ++i) o.v[i] = ld2(&r.v[2 * i]);
+  return o;
+}
+template <class IO, int W>
+__device__ __forceinline__ Row<IO, W> load(const IO* p, int nc, bool fast) {
+  if (fast) return widen<IO, W>(*reinterpret_cast<const Vec<IO, W>*>(p));
+  Row<IO, W> o;
+#pragma unroll
+  for (int i = 0; i < W / 2; ++i) o.v[i] = pk(2 * i < nc ? to_f(p[2 * i]) : 0.f, 2 * i + 1 < nc ? to_f(p[2 * i + 1]) : 0.f);
+  return o;
+}
+template <class IO, int W>
+__device__ __forceinline__ void store(IO* p, const Row<IO, W>& r, int nc, bool fast) {
+  if (fast) {
+    Vec<IO, W> o;
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) st2(&o.v[2 * i], r.v[i]);
+    *reinterpret_cast<Vec<IO, W>*>(p) = o;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+    if (i < nc) from_f(p[i], i % 2 ? up(r.v[i / 2]).y : up(r.v[i / 2]).x);
+}
+template <class IO, int W>
+__device__ __forceinline__ Row<IO, W> zeros() {
+  Row<IO, W> o;
+#pragma unroll
+  for (int i = 0; i < W / 2; ++i) o.v[i] = 0;
+  return o;
 }
 
-// grid (channel blocks, batch x time CTAs)
+// A thread's place: W channels from c, steps t0 .. t0 + n - 1 of row b, of which `live` are before the row's length
+// (more or fewer than n, or none: the values beside the run matter only up to K away).
+template <int K, class IO, int W>
+struct Run {
+  int64_t b, c, t0, len;
+  int r, n, live, nc;
+  bool fast;
+  const IO *x, *init;
+  __device__ __forceinline__ explicit Run(const ConvArgs& a) {
+    c = ((int64_t)blockIdx.y * 32 + (threadIdx.x & 31)) * W;
+    nc = c >= a.C ? 0 : a.C - c < W ? (int)(a.C - c) : W;
+    b = blockIdx.x / a.ygrid;
+    r = (int)(blockIdx.x - b * a.ygrid) * kConvWarps + (threadIdx.x >> 5);
+    len = row_len(a.len, (int)b, a.T);
+    t0 = (int64_t)r * a.run;
+    n = a.T - t0 < a.run ? (a.T - t0 < 0 ? 0 : (int)(a.T - t0)) : a.run;
+    const int64_t l = len - t0;
+    live = l < -K ? -K : l > a.run + K ? a.run + K : (int)l;
+    fast = a.vec && nc == W;
+    x = (const IO*)a.x + b * a.x_sb + c;
+    init = a.init ? (const IO*)a.init + b * (K - 1) * a.C + c : nullptr;
+  }
+  // step t of the row (t >= -(K - 1)), the state where t < 0
+  __device__ __forceinline__ Row<IO, W> at(const ConvArgs& a, int64_t t) const {
+    if (t >= 0) return load<IO, W>(x + t * a.x_st, nc, fast);
+    if (init) return load<IO, W>(init + (t + K - 1) * a.C, nc, fast);
+    return zeros<IO, W>();
+  }
+  __device__ __forceinline__ void taps(const ConvArgs& a, f2 (&w)[K][W / 2], f2 (&bias)[W / 2]) const {
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+      const bool o0 = 2 * i < nc, o1 = 2 * i + 1 < nc;
+      const int64_t k = c + 2 * i;
+      bias[i] = pk(a.bias && o0 ? a.bias[k] : 0.f, a.bias && o1 ? a.bias[k + 1] : 0.f);
+#pragma unroll
+      for (int j = 0; j < K; ++j) w[j][i] = pk(o0 ? a.w[k * K + j] : 0.f, o1 ? a.w[(k + 1) * K + j] : 0.f);
+    }
+  }
+};
+
+// grid (batch x time CTAs, channel blocks)
 template <int K, class IO, int W>
 __global__ void __launch_bounds__(32 * kConvWarps) k_causal_conv_fwd(const ConvArgs a) {
-  const int64_t c = ((int64_t)blockIdx.y * 32 + (threadIdx.x & 31)) * W;
+  constexpr int P = W / 2;
+  const Run<K, IO, W> q(a);
+  if (q.nc == 0) return;
+  if (q.r == 0) {  // the last K - 1 inputs of the row
+    IO* f = (IO*)a.final_state + q.b * (K - 1) * a.C + q.c;
+#pragma unroll
+    for (int i = 0; i < K - 1; ++i) store<IO, W>(f + i * a.C, q.at(a, q.len + i - (K - 1)), q.nc, q.fast);
+  }
+  if (q.n == 0) return;
+  IO* y = (IO*)a.y + (q.b * a.T + q.t0) * a.C + q.c;
+  f2 w[K][P], bias[P], win[K][P];  // win[j]: step t + j - (K - 1)
+  q.taps(a, w, bias);
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) {
+    const Row<IO, W> v = q.live > 0 ? q.at(a, q.t0 + j - (K - 1)) : zeros<IO, W>();
+#pragma unroll
+    for (int i = 0; i < P; ++i) win[j][i] = v.v[i];
+  }
+  auto step = [&](const Row<IO, W>& in) {
+    Row<IO, W> o;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      win[K - 1][i] = in.v[i];
+      f2 s = bias[i];
+#pragma unroll
+      for (int j = 0; j < K; ++j) s = fma2(w[j][i], win[j][i], s);
+      o.v[i] = a.silu ? mul2(s, sigmoid_2(s)) : s;
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) win[j][i] = win[j + 1][i];
+    }
+    return o;
+  };
+  const IO* x = q.x + q.t0 * a.x_st;
+  const int nl = q.n < q.live ? q.n : q.live;
+  int t = 0;
+  if (q.fast)
+    for (; t + kConvU <= nl; t += kConvU) {
+      Vec<IO, W> in[kConvU];
+#pragma unroll
+      for (int k = 0; k < kConvU; ++k) in[k] = *reinterpret_cast<const Vec<IO, W>*>(x + (t + k) * a.x_st);
+#pragma unroll
+      for (int k = 0; k < kConvU; ++k) store<IO, W>(y + (t + k) * a.C, step(widen<IO, W>(in[k])), W, true);
+    }
+#pragma unroll 2
+  for (; t < nl; ++t) store<IO, W>(y + t * a.C, step(load<IO, W>(x + t * a.x_st, q.nc, q.fast)), q.nc, q.fast);
+  for (; t < q.n; ++t) store<IO, W>(y + t * a.C, zeros<IO, W>(), q.nc, q.fast);
+}
+
+// One step (T = 1): a thread reads its channels' K - 1 carried inputs and the new one once, and writes y and the shifted
+// state. grid (channel blocks, batch).
+constexpr int kConvStepThr = 128;
+template <int K, class IO, int W>
+__global__ void __launch_bounds__(kConvStepThr) k_causal_conv_step(const ConvArgs a) {
+  constexpr int P = W / 2;
+  const int64_t b = blockIdx.y, c = ((int64_t)blockIdx.x * kConvStepThr + threadIdx.x) * W;
   if (c >= a.C) return;
   const int nc = a.C - c < W ? (int)(a.C - c) : W;
-  const int64_t b = blockIdx.x / a.ygrid, r = (blockIdx.x - b * a.ygrid) * kConvWarps + (threadIdx.x >> 5);
-  const int64_t len = row_len(a.len, (int)b, a.T);
-  const int64_t t0 = r * a.run, t1 = t0 + a.run < a.T ? t0 + a.run : a.T;
-  const IO* x = (const IO*)a.x + b * a.x_sb;
-  const IO* init = a.init ? (const IO*)a.init + b * (K - 1) * a.C : nullptr;
-  if (r == 0) {  // the last K - 1 inputs of the row
-    IO* f = (IO*)a.final_state + b * (K - 1) * a.C + c;
+  const bool fast = a.vec && nc == W, live = row_len(a.len, (int)b, 1) > 0;
+  Row<IO, W> v[K];
 #pragma unroll
-    for (int i = 0; i < K - 1; ++i)
-      store_row<IO, W>(f + i * a.C, 0, nc, a.vec, step_row<K, IO, W>(a, x, init, len + i - (K - 1), c, nc));
+  for (int j = 0; j < K - 1; ++j)
+    v[j] = a.init ? load<IO, W>((const IO*)a.init + (b * (K - 1) + j) * a.C + c, nc, fast) : zeros<IO, W>();
+  v[K - 1] = live ? load<IO, W>((const IO*)a.x + b * a.x_sb + c, nc, fast) : zeros<IO, W>();
+  IO* f = (IO*)a.final_state + b * (K - 1) * a.C + c;
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) store<IO, W>(f + j * a.C, live ? v[j + 1] : v[j], nc, fast);
+  Row<IO, W> o;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const bool o0 = 2 * i < nc, o1 = 2 * i + 1 < nc;
+    const int64_t k = c + 2 * i;
+    f2 s = pk(a.bias && o0 ? a.bias[k] : 0.f, a.bias && o1 ? a.bias[k + 1] : 0.f);
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      s = fma2(pk(o0 ? a.w[k * K + j] : 0.f, o1 ? a.w[(k + 1) * K + j] : 0.f), v[j].v[i], s);
+    o.v[i] = a.silu ? mul2(s, sigmoid_2(s)) : s;
   }
-  if (t0 >= a.T) return;
-  IO* y = (IO*)a.y + b * a.T * a.C + c;
-  float w[K][W], bias[W], win[K][W];
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
-    bias[i] = a.bias && i < nc ? a.bias[c + i] : 0.f;
-#pragma unroll
-    for (int j = 0; j < K; ++j) w[j][i] = i < nc ? a.w[(c + i) * K + j] : 0.f;
-  }
-  if (t0 < len) {
-#pragma unroll
-    for (int j = 0; j < K - 1; ++j) {
-      const Vec<IO, W> v = step_row<K, IO, W>(a, x, init, t0 + j - (K - 1), c, nc);
-#pragma unroll
-      for (int i = 0; i < W; ++i) win[j][i] = to_f(v.v[i]);
-    }
-  }
-  for (int64_t t = t0; t < t1; t += kConvU) {
-    Vec<IO, W> in[kConvU];
-#pragma unroll
-    for (int k = 0; k < kConvU; ++k)
-      in[k] = t + k < t1 && t + k < len ? load_row<IO, W>(x + (t + k) * a.x_st + c, 0, nc, a.vec) : zero_row<IO, W>();
-#pragma unroll
-    for (int k = 0; k < kConvU; ++k) {
-      if (t + k >= t1) break;
-      Vec<IO, W> o = zero_row<IO, W>();
-      if (t + k < len) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          win[K - 1][i] = to_f(in[k].v[i]);
-          float s = bias[i];
-#pragma unroll
-          for (int j = 0; j < K; ++j) s = fmaf(w[j][i], win[j][i], s);
-          if (a.silu) s *= sigmoid(s);
-          from_f(o.v[i], s);
-#pragma unroll
-          for (int j = 0; j < K - 1; ++j) win[j][i] = win[j + 1][i];
-        }
-      }
-      store_row<IO, W>(y + (t + k) * a.C, 0, nc, a.vec, o);
-    }
-  }
+  store<IO, W>((IO*)a.y + b * a.C + c, live ? o : zeros<IO, W>(), nc, fast);
 }
 
 template <int K, class IO, int W>
 __global__ void __launch_bounds__(32 * kConvWarps) k_causal_conv_bwd(const ConvArgs a) {
+  constexpr int P = W / 2;
   __shared__ float s_red[kConvWarps][32][W * (K + 1) + 1];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = ((int64_t)blockIdx.y * 32 + lane) * W;
-  const int nc = c >= a.C ? 0 : a.C - c < W ? (int)(a.C - c) : W;
-  const int64_t b = blockIdx.x / a.ygrid, yb = blockIdx.x - b * a.ygrid, r = yb * kConvWarps + warp;
-  const int64_t len = row_len(a.len, (int)b, a.T);
-  const int64_t t0 = r * a.run, t1 = t0 + a.run < a.T ? t0 + a.run : a.T;
-  float acc[K][W], accb[W];
+  const Run<K, IO, W> q(a);
+  f2 acc[K][P], accb[P];
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    accb[i] = 0.f;
+  for (int i = 0; i < P; ++i) {
+    accb[i] = 0;
 #pragma unroll
-    for (int j = 0; j < K; ++j) acc[j][i] = 0.f;
+    for (int j = 0; j < K; ++j) acc[j][i] = 0;
   }
-  if (nc > 0 && t0 < a.T) {
-    const IO* x = (const IO*)a.x + b * a.x_sb;
-    const IO* dy = (const IO*)a.dy + b * a.dy_sb + c;
-    const IO* init = a.init ? (const IO*)a.init + b * (K - 1) * a.C : nullptr;
-    const IO* df = a.d_final ? (const IO*)a.d_final + b * (K - 1) * a.C + c : nullptr;
-    IO* dx = (IO*)a.dx + b * a.T * a.C + c;
-    IO* di = a.d_init ? (IO*)a.d_init + b * (K - 1) * a.C + c : nullptr;
-    float w[K][W], bias[W], win[K][W], dp[K][W];  // dp[j]: step t - j
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      bias[i] = a.bias && i < nc ? a.bias[c + i] : 0.f;
-#pragma unroll
-      for (int j = 0; j < K; ++j) {
-        w[j][i] = i < nc ? a.w[(c + i) * K + j] : 0.f;
-        dp[j][i] = 0.f;
-      }
-    }
+  if (q.nc > 0 && q.n > 0) {
+    const IO* x = q.x + q.t0 * a.x_st;
+    const IO* dy = (const IO*)a.dy + q.b * a.dy_sb + q.t0 * a.dy_st + q.c;
+    const IO* df = a.d_final ? (const IO*)a.d_final + q.b * (K - 1) * a.C + q.c : nullptr;
+    IO* dx = (IO*)a.dx + (q.b * a.T + q.t0) * a.C + q.c;
+    IO* di = a.d_init && q.r == 0 ? (IO*)a.d_init + q.b * (K - 1) * a.C + q.c : nullptr;
+    f2 w[K][P], bias[P], win[K][P], dp[K][P];  // dp[j]: the gradient of pre at step t - j
+    q.taps(a, w, bias);
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) {
-      const Vec<IO, W> v = t0 + j - (K - 1) < len ? step_row<K, IO, W>(a, x, init, t0 + j - (K - 1), c, nc)
-                                                  : zero_row<IO, W>();
+      const Row<IO, W> v = j - (K - 1) < q.live ? q.at(a, q.t0 + j - (K - 1)) : zeros<IO, W>();
 #pragma unroll
-      for (int i = 0; i < W; ++i) win[j][i] = to_f(v.v[i]);
+      for (int i = 0; i < P; ++i) win[j][i] = v.v[i];
     }
-    const int64_t tend = t1 + K - 1;
-    for (int64_t t = t0; t < tend; t += kConvU) {
-      Vec<IO, W> in[kConvU], up[kConvU];
 #pragma unroll
-      for (int k = 0; k < kConvU; ++k) {
-        const bool live = t + k < tend && t + k < len;
-        in[k] = live ? load_row<IO, W>(x + (t + k) * a.x_st + c, 0, nc, a.vec) : zero_row<IO, W>();
-        up[k] = live ? load_row<IO, W>(dy + (t + k) * a.dy_st, 0, nc, a.vec) : zero_row<IO, W>();
-      }
+    for (int j = 0; j < K; ++j)
 #pragma unroll
-      for (int k = 0; k < kConvU; ++k) {
-        if (t + k >= tend) break;
-        const int64_t s = t + k - (K - 1);
-        Vec<IO, W> extra = zero_row<IO, W>();  // the gradient of the final state, where step s is in it
-        const int64_t at = s - (len - (K - 1));
-        if (df && at >= 0 && at < K - 1) extra = load_row<IO, W>(df + at * a.C, 0, nc, a.vec);
-        Vec<IO, W> o;
+      for (int i = 0; i < P; ++i) dp[j][i] = 0;
+    // one step; the gradient it completes is step t - (K - 1)'s. own: counts for dw
+    auto step = [&](const Row<IO, W>& in, const Row<IO, W>& up_, bool own) {
+      Row<IO, W> o;
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-          win[K - 1][i] = to_f(in[k].v[i]);
-          float d = to_f(up[k].v[i]);
-          if (a.silu) {
-            float p = bias[i];
+      for (int i = 0; i < P; ++i) {
+        win[K - 1][i] = in.v[i];
+        f2 d = up_.v[i];
+        if (a.silu) {
+          f2 p = bias[i];
 #pragma unroll
-            for (int j = 0; j < K; ++j) p = fmaf(w[j][i], win[j][i], p);
-            const float sg = sigmoid(p);
-            // slope of silu; where e^-p overflows sg is 0 and so is the slope
-            d *= sg * fmaf(p, 1.f - sg, 1.f);
-          }
-          if (t + k >= len) d = 0.f;
-#pragma unroll
-          for (int j = K - 1; j > 0; --j) dp[j][i] = dp[j - 1][i];
-          dp[0][i] = d;
-          if (t + k < t1) {
-            accb[i] += d;
-#pragma unroll
-            for (int j = 0; j < K; ++j) acc[j][i] = fmaf(d, win[j][i], acc[j][i]);
-          }
-          float g = to_f(extra.v[i]);
-#pragma unroll
-          for (int j = 0; j < K; ++j) g = fmaf(w[j][i], dp[j][i], g);
-          from_f(o.v[i], s < len ? g : 0.f);
-#pragma unroll
-          for (int j = 0; j < K - 1; ++j) win[j][i] = win[j + 1][i];
+          for (int j = 0; j < K; ++j) p = fma2(w[j][i], win[j][i], p);
+          // slope of silu: sg (1 + p (1 - sg))
+          const f2 sg = sigmoid_2(p);
+          d = mul2(mul2(d, sg), fma2(p, fma2(sg, both(-1.f), both(1.f)), both(1.f)));
         }
-        if (s >= t0 && s < t1) store_row<IO, W>(dx + s * a.C, 0, nc, a.vec, o);
-        else if (s < 0 && di) store_row<IO, W>(di + (s + K - 1) * a.C, 0, nc, a.vec, o);
+#pragma unroll
+        for (int j = K - 1; j > 0; --j) dp[j][i] = dp[j - 1][i];
+        dp[0][i] = d;
+        if (own) {
+          accb[i] = add2(accb[i], d);
+#pragma unroll
+          for (int j = 0; j < K; ++j) acc[j][i] = fma2(d, win[j][i], acc[j][i]);
+        }
+        f2 g = mul2(w[0][i], dp[0][i]);
+#pragma unroll
+        for (int j = 1; j < K; ++j) g = fma2(w[j][i], dp[j][i], g);
+        o.v[i] = g;
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) win[j][i] = win[j + 1][i];
       }
-    }
+      return o;
+    };
+    // a step anywhere: past the length, before the run, the gradient of the final state
+    auto edge = [&](int t) {
+      const bool on = t < q.live;
+      Row<IO, W> o = step(on ? load<IO, W>(x + t * a.x_st, q.nc, q.fast) : zeros<IO, W>(),
+                          on ? load<IO, W>(dy + t * a.dy_st, q.nc, q.fast) : zeros<IO, W>(), on && t < q.n);
+      const int s = t - (K - 1), at = s - (q.live - (K - 1));
+      if (s >= q.live) o = zeros<IO, W>();
+      else if (df && at >= 0) {
+        const Row<IO, W> e = load<IO, W>(df + at * a.C, q.nc, q.fast);
+#pragma unroll
+        for (int i = 0; i < P; ++i) o.v[i] = add2(o.v[i], e.v[i]);
+      }
+      if (s >= 0 && s < q.n) store<IO, W>(dx + s * a.C, o, q.nc, q.fast);
+      else if (s < 0 && di) store<IO, W>(di + (s + K - 1) * a.C, o, q.nc, q.fast);
+    };
+    const int nl = q.n < q.live ? q.n : q.live;
+    int t = 0;
+#pragma unroll 1
+    for (; t < K - 1; ++t) edge(t);  // complete gradients of the run before, or of the initial state
+    if (q.fast)
+      for (; t + kConvU <= nl; t += kConvU) {
+        Vec<IO, W> in[kConvU], up_[kConvU];
+#pragma unroll
+        for (int k = 0; k < kConvU; ++k) {
+          in[k] = *reinterpret_cast<const Vec<IO, W>*>(x + (t + k) * a.x_st);
+          up_[k] = *reinterpret_cast<const Vec<IO, W>*>(dy + (t + k) * a.dy_st);
+        }
+#pragma unroll
+        for (int k = 0; k < kConvU; ++k)
+          store<IO, W>(dx + (t + k - (K - 1)) * a.C, step(widen<IO, W>(in[k]), widen<IO, W>(up_[k]), true), W, true);
+      }
+#pragma unroll 1
+    for (; t < q.n + K - 1; ++t) edge(t);
   }
 #pragma unroll
   for (int i = 0; i < W; ++i) {
+    auto half = [&](f2 v) { return i % 2 ? up(v).y : up(v).x; };
 #pragma unroll
-    for (int j = 0; j < K; ++j) s_red[warp][lane][i * (K + 1) + j] = acc[j][i];
-    s_red[warp][lane][i * (K + 1) + K] = accb[i];
+    for (int j = 0; j < K; ++j) s_red[threadIdx.x >> 5][threadIdx.x & 31][i * (K + 1) + j] = half(acc[j][i / 2]);
+    s_red[threadIdx.x >> 5][threadIdx.x & 31][i * (K + 1) + K] = half(accb[i / 2]);
   }
   __syncthreads();
   // record of this CTA: 32 W channels x (K + 1), channel-major like w
@@ -212,7 +320,7 @@ __global__ void __launch_bounds__(32 * kConvWarps) k_causal_conv_bwd(const ConvA
     const int ln = e / (W * (K + 1)), k = e - ln * (W * (K + 1));
     float s = 0.f;
 #pragma unroll
-    for (int q = 0; q < kConvWarps; ++q) s += s_red[q][ln][k];
+    for (int u = 0; u < kConvWarps; ++u) s += s_red[u][ln][k];
     out[e] = s;
   }
 }

@@ -13,7 +13,7 @@ enum KernelId {
   KID_BWD_GRADS, KID_BWD_BUFOUT, KID_BWD_FINAL, KID_BWD_DSREF, KID_FMAP_BWD, KID_FWD_CHUNK_TC, KID_FWD_OUT_TC, KID_FWD_BUF_Y,
   KID_BWD_CHUNK_TC, KID_BWD_STATE_GATES_TC, KID_BWD_BUF_TC, KID_BWD_FINAL_TC, KID_BWD_DSREF_TC, KID_BWD_KEYS_TC, KID_SREF_TILE, KID_DECODE, KID_SCAN_OP_FWD, KID_SCAN_OP_BWD, KID_CARRY, KID_DWCONV_FWD, KID_DWCONV_BWD, KID_HEADPREP_FWD, KID_HEADPREP_BWD, KID_PROJ_TILES, KID_FMAP_FWD_TC, KID_FMAP_BWD_TC, KID_OMEGA_STORE_FWD, KID_OMEGA_STORE_BWD, KID_AFFINE_FWD, KID_AFFINE_BWD,
   KID_SSCAN_FWD, KID_SSCAN_ENDS, KID_SSCAN_CARRY, KID_SSCAN_STEP, KID_SSCAN_BWD, KID_SSCAN_BWD_ENDS, KID_SSCAN_DBC, KID_SSCAN_DA,
-  KID_CONV_FWD, KID_CONV_BWD, KID_CONV_DW, KID_SAMPLE, KID_DISTILL_FWD, KID_DISTILL_BWD, KID_COUNT
+  KID_CONV_FWD, KID_CONV_STEP, KID_CONV_BWD, KID_CONV_DW, KID_SAMPLE, KID_DISTILL_FWD, KID_DISTILL_BWD, KID_COUNT
 };
 
 int prof_begin(int kid, cudaStream_t st);

@@ -155,9 +155,13 @@ int step_t(const AtlasSelScan* a, ScanArgs s, cudaStream_t st) {
   alignment(a, s, 4);
   const int vec4 = a->N % 4 == 0 && (uintptr_t)a->A % 16 == 0 && (uintptr_t)a->h0 % 16 == 0 &&
                    (uintptr_t)a->hT % 16 == 0;
-  const int64_t per = kStepThr / (NP / 4), grid = (a->B * a->D + per - 1) / per;
-  if (grid > 0x7fffffff) return ATLAS_ERR_UNSUPPORTED;
-  LAUNCH_T(KID_SSCAN_STEP, (k_sscan_step<IO, NP>), dim3((unsigned)grid), kStepThr, 0, st, s, vec4);
+  // four rows a thread while that still leaves two waves of threads
+  const int64_t per = kStepThr / (NP / 4), gx = (a->D + per - 1) / per, rows = a->B * gx >= 8 * 4 * 148 * 2 ? 4 : 1;
+  const int64_t gy = (a->B + rows - 1) / rows;
+  if (gx > 0x7fffffff || gy > 65535) return ATLAS_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)gx, (unsigned)gy);
+  if (rows == 4) LAUNCH_T(KID_SSCAN_STEP, (k_sscan_step<IO, NP, 4>), grid, kStepThr, 0, st, s, vec4);
+  else LAUNCH_T(KID_SSCAN_STEP, (k_sscan_step<IO, NP, 1>), grid, kStepThr, 0, st, s, vec4);
   return ATLAS_OK;
 }
 
@@ -188,7 +192,7 @@ int bwd_t(const AtlasSelScan* a, ScanArgs s, const BwdLayout& L, cudaStream_t st
 
 template <class IO>
 int fwd_io(const AtlasSelScan* a, const Plan& p, const ScanArgs& s, cudaStream_t st) {
-  if (a->T == 1 && !s.hsave) {
+  if (a->T == 1 && !s.hsave && a->B <= 65535) {
     switch (p.np) {
       case 8: return step_t<IO, 8>(a, s, st);
       case 16: return step_t<IO, 16>(a, s, st);

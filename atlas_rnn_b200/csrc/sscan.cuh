@@ -406,70 +406,87 @@ __global__ void __launch_bounds__(kCarryThr) k_sscan_carry(const ScanArgs a) {
 }
 
 // ---- one token ------------------------------------------------------------
-// T = 1 without a backward: a thread takes 4 neighbouring states (one 16-byte read and write of the
-// state, which is the traffic), LPC = NP / 4 lanes a channel.
+// T = 1 without a backward: a thread takes 4 neighbouring states (one 16-byte read and write of the state, which is the
+// traffic) of R batch rows, whose loads are all in flight together; LPC = NP / 4 lanes a channel. A, D and bias are read
+// once for the R rows. grid (channel blocks, row blocks).
 constexpr int kStepThr = 128;
-template <class IO, int NP>
+template <class IO, int NP, int R>
 __global__ void __launch_bounds__(kStepThr) k_sscan_step(const ScanArgs a, int vec4) {
   constexpr int LPC = NP / 4;
-  const int64_t at = (int64_t)blockIdx.x * (kStepThr / LPC) + threadIdx.x / LPC;  // b * Dm + d
-  const int l = threadIdx.x % LPC;
-  const bool mine = at < (int64_t)a.Bsz * a.Dm;
-  const int b = mine ? (int)(at / a.Dm) : 0, d = mine ? (int)(at % a.Dm) : 0, g = d / (a.Dm / a.G);
-  const bool live = mine && row_len(a.len, b, 1) > 0;
-  float Av[4] = {0.f, 0.f, 0.f, 0.f}, hv[4] = {0.f, 0.f, 0.f, 0.f};
-  if (mine) {
-    const float *Ap = a.A + (int64_t)d * a.N + l * 4, *hp = a.h0 ? a.h0 + at * a.N + l * 4 : nullptr;
-    if (vec4) {
-      if (l * 4 < a.N) {
-        const float4 x = *reinterpret_cast<const float4*>(Ap);
-        Av[0] = x.x, Av[1] = x.y, Av[2] = x.z, Av[3] = x.w;
-        if (hp) {
-          const float4 y = *reinterpret_cast<const float4*>(hp);
-          hv[0] = y.x, hv[1] = y.y, hv[2] = y.z, hv[3] = y.w;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (l * 4 + i < a.N) {
-          Av[i] = Ap[i];
-          if (hp) hv[i] = hp[i];
-        }
-    }
-  }
-  float dt = 0.f, uu = 0.f, zz = 0.f;
-  Vec<IO, 4> Bv = zero_row<IO, 4>(), Cv = Bv;
-  if (live) {
-    uu = to_f(((const IO*)a.u)[b * a.u_sb + d]);
-    dt = to_f(((const IO*)a.delta)[b * a.d_sb + d]) + (a.bias ? a.bias[d] : 0.f);
-    if (a.z) zz = to_f(((const IO*)a.z)[b * a.z_sb + d]);
-    if (a.softplus) dt = softplus(dt);
-    Bv = load_row<IO, 4>((const IO*)a.Bm + b * a.B_sb + g * a.B_sg, l * 4, a.N, a.vecbc);
-    Cv = load_row<IO, 4>((const IO*)a.Cm + b * a.C_sb + g * a.C_sg, l * 4, a.N, a.vecbc);
-  }
-  float y = 0.f;
-  const float dl = dt * kLog2e, du = dt * uu;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    hv[i] = fmaf(ex2(Av[i] * dl), hv[i], du * to_f(Bv.v[i]));
-    y = fmaf(to_f(Cv.v[i]), hv[i], y);
-  }
-#pragma unroll
-  for (int o = LPC / 2; o >= 1; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-  if (!mine) return;
-  float* ho = a.hT + at * a.N + l * 4;
-  if (vec4) {
-    if (l * 4 < a.N) *reinterpret_cast<float4*>(ho) = make_float4(hv[0], hv[1], hv[2], hv[3]);
+  const int d = blockIdx.x * (kStepThr / LPC) + threadIdx.x / LPC, n4 = threadIdx.x % LPC * 4;
+  const bool on = d < a.Dm;
+  const int dd = on ? d : 0, g = dd / (a.Dm / a.G);
+  const bool v4 = vec4 && n4 < a.N;
+  float A[4] = {0.f, 0.f, 0.f, 0.f}, h[R][4];
+  float dt[R], u[R], z[R];
+  Vec<IO, 4> B[R], C[R];
+  bool live[R];
+  const float* Ap = a.A + (int64_t)dd * a.N + n4;
+  if (v4) {
+    const float4 x = *reinterpret_cast<const float4*>(Ap);
+    A[0] = x.x, A[1] = x.y, A[2] = x.z, A[3] = x.w;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (l * 4 + i < a.N) ho[i] = hv[i];
+      if (n4 + i < a.N) A[i] = Ap[i];
   }
-  if (l == 0) {
-    if (a.D) y = fmaf(a.D[d], uu, y);
-    if (a.z) y *= zz * sigmoid(zz);
-    from_f(((IO*)a.out)[at], live ? y : 0.f);
+  const float bias = a.bias ? a.bias[dd] : 0.f, skip = a.D ? a.D[dd] : 0.f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t b = (int64_t)blockIdx.y * R + r;
+    const bool row = on && b < a.Bsz;
+    live[r] = row && row_len(a.len, (int)(row ? b : 0), 1) > 0;
+    const int64_t at = (row ? b * a.Dm + d : 0) * a.N + n4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[r][i] = 0.f;
+    if (row && a.h0) {
+      if (v4) {
+        const float4 x = *reinterpret_cast<const float4*>(a.h0 + at);
+        h[r][0] = x.x, h[r][1] = x.y, h[r][2] = x.z, h[r][3] = x.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n4 + i < a.N) h[r][i] = a.h0[at + i];
+      }
+    }
+    u[r] = dt[r] = z[r] = 0.f;
+    B[r] = C[r] = zero_row<IO, 4>();
+    if (live[r]) {
+      u[r] = to_f(((const IO*)a.u)[b * a.u_sb + d]);
+      dt[r] = to_f(((const IO*)a.delta)[b * a.d_sb + d]);
+      if (a.z) z[r] = to_f(((const IO*)a.z)[b * a.z_sb + d]);
+      B[r] = load_row<IO, 4>((const IO*)a.Bm + b * a.B_sb + g * a.B_sg, n4, a.N, a.vecbc);
+      C[r] = load_row<IO, 4>((const IO*)a.Cm + b * a.C_sb + g * a.C_sg, n4, a.N, a.vecbc);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t b = (int64_t)blockIdx.y * R + r;
+    float x = dt[r] + bias, y = 0.f;
+    if (a.softplus) x = softplus(x);
+    if (!live[r]) x = 0.f;
+    const float xl = x * kLog2e, du = x * u[r];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[r][i] = fmaf(ex2(A[i] * xl), h[r][i], du * to_f(B[r].v[i]));
+      y = fmaf(to_f(C[r].v[i]), h[r][i], y);
+    }
+#pragma unroll
+    for (int o = LPC / 2; o >= 1; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    if (!on || b >= a.Bsz) continue;
+    float* ho = a.hT + (b * a.Dm + d) * a.N + n4;
+    if (v4) {
+      *reinterpret_cast<float4*>(ho) = make_float4(h[r][0], h[r][1], h[r][2], h[r][3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n4 + i < a.N) ho[i] = h[r][i];
+    }
+    if (n4 == 0) {
+      y = fmaf(skip, u[r], y);
+      if (a.z) y *= z[r] * sigmoid(z[r]);
+      from_f(((IO*)a.out)[b * a.Dm + d], live[r] ? y : 0.f);
+    }
   }
 }
 

@@ -10,6 +10,7 @@ No reference counterpart.
 """
 from __future__ import annotations
 
+import ctypes
 import struct
 
 import torch
@@ -17,7 +18,6 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _stream
 
 MAX_STATE = 64     # states per channel
 MAX_CONV_K = 8     # taps
@@ -38,8 +38,8 @@ def _need_cuda(t: Tensor, what: str):
 
 
 def _check(what: str, name: str, t: Tensor, shape: tuple, dtype, device):
-    if tuple(t.shape) != shape:
-        raise ValueError(f"atlas_rnn_b200.{what}: {name} must have shape {shape}, not {tuple(t.shape)}")
+    if t.shape != shape:
+        raise ValueError(f"atlas_rnn_b200.{what}: {name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"atlas_rnn_b200.{what}: {name} must be {dtype}, not {t.dtype}")
     if t.device != device:
@@ -50,10 +50,12 @@ def _f32(what: str, name: str, t: Tensor | None, shape: tuple, device) -> Tensor
     """A parameter or state as dense fp32."""
     if t is None:
         return None
-    if not t.is_floating_point():
-        raise TypeError(f"atlas_rnn_b200.{what}: {name} must be a floating type, not {t.dtype}")
     _check(what, name, t, shape, None, device)
-    return t.to(torch.float32).contiguous()
+    if t.dtype != torch.float32:
+        if not t.is_floating_point():
+            raise TypeError(f"atlas_rnn_b200.{what}: {name} must be a floating type, not {t.dtype}")
+        t = t.to(torch.float32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _rows(t: Tensor) -> Tensor:
@@ -71,12 +73,22 @@ def _lengths(what: str, lengths, batch: int, device) -> Tensor | None:
         else lengths.contiguous()
 
 
-def _run(device, call):
-    """``call`` with ``device`` current (kernels launch on the current device)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return call()
-    with torch.cuda.device(device):
-        return call()
+def _wants_grad(*tensors) -> bool:
+    if not torch.is_grad_enabled():
+        return False
+    return any(t is not None and t.requires_grad for t in tensors)
+
+
+def _run(what: str, fn, device, *args):
+    """fn(*args, current stream of device) with ``device`` current: kernels launch on the current device."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        _lib.check(code, what)
 
 
 # ---- selective scan --------------------------------------------------------------------------
@@ -104,7 +116,6 @@ class _Scan:
             _ptr(du), _ptr(ddelta), _ptr(dz), _ptr(dB), _ptr(dC), _ptr(dA), _ptr(dD), _ptr(dbias), _ptr(dh0))
 
     def workspaces(self):
-        import ctypes
         s, f, b = ctypes.c_size_t(), ctypes.c_size_t(), ctypes.c_size_t()
         _lib.check(_lib.lib().atlas_sscan_workspace(self.pack(), ctypes.byref(s), ctypes.byref(f), ctypes.byref(b)),
                    "selective_scan workspace")
@@ -121,8 +132,7 @@ class _Scan:
             ns, nf, _ = self.workspaces()
             saved = torch.empty(ns, dtype=torch.uint8, device=dev) if keep else None
             scratch = torch.empty(nf, dtype=torch.uint8, device=dev) if nf else None
-        _lib.check(_run(dev, lambda: _lib.lib().atlas_sscan_forward(self.pack(out, hT, saved, scratch),
-                                                                    _stream(dev))), "selective_scan forward")
+        _run("selective_scan forward", _lib.lib().atlas_sscan_forward, dev, self.pack(out, hT, saved, scratch))
         return out, hT, saved
 
 
@@ -154,8 +164,7 @@ class SelectiveScanFn(torch.autograd.Function):
         scratch = torch.empty(s.workspaces()[2], dtype=torch.uint8, device=dev)
         packed = s.pack(saved=saved, scratch=scratch, dout=dout, dhT=dhT, du=du, ddelta=ddelta, dz=dz, dB=dB, dC=dC,
                         dA=dA, dD=dD, dbias=dbias, dh0=dh0)
-        _lib.check(_run(dev, lambda: _lib.lib().atlas_sscan_backward(packed, _stream(dev))),
-                   "selective_scan backward")
+        _run("selective_scan backward", _lib.lib().atlas_sscan_backward, dev, packed)
         return du, ddelta, dA, dB, dC, dD, dz, dbias, dh0, None, None, None
 
 
@@ -216,7 +225,7 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D:
         return _no_steps(u, n, h0)
     u, delta, B, C = _rows(u), _rows(delta), _rows(B), _rows(C)
     z = None if z is None else _rows(z)
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (u, delta, A, B, C, D, z, bias, h0)):
+    if _wants_grad(u, delta, A, B, C, D, z, bias, h0):
         return SelectiveScanFn.apply(u, delta, A, B, C, D, z, bias, h0, lengths, bool(delta_softplus), chunk)
     out, hT, _ = _Scan(u, delta, A, B, C, D, z, bias, h0, lengths, bool(delta_softplus), chunk).forward(keep=False)
     return out, hT
@@ -229,9 +238,9 @@ def _conv_forward(x, w, bias, init, lengths, silu):
     K = w.shape[1]
     y = torch.empty(B, T, C, dtype=x.dtype, device=x.device)
     final = torch.empty(B, K - 1, C, dtype=x.dtype, device=x.device)
-    _lib.check(_run(x.device, lambda: _lib.lib().atlas_causal_conv_forward(
-        _ptr(x), x.stride(0), x.stride(1), _ptr(w), _ptr(bias), _ptr(init), _ptr(lengths), _ptr(y), _ptr(final), K,
-        silu, _IO[x.dtype], B, T, C, _stream(x.device))), "causal_conv1d forward")
+    _run("causal_conv1d forward", _lib.lib().atlas_causal_conv_forward, x.device, x.data_ptr(), x.stride(0),
+         x.stride(1), w.data_ptr(), _ptr(bias), _ptr(init), _ptr(lengths), y.data_ptr(), final.data_ptr(), K, silu,
+         _IO[x.dtype], B, T, C)
     return y, final
 
 
@@ -259,10 +268,10 @@ class CausalConv1dFn(torch.autograd.Function):
         dbias = torch.empty(C, dtype=torch.float32, device=dev) if bias is not None else None
         L = _lib.lib()
         scratch = torch.empty(L.atlas_causal_conv_scratch(B, T, C, K), dtype=torch.uint8, device=dev)
-        _lib.check(_run(dev, lambda: L.atlas_causal_conv_backward(
-            _ptr(x), x.stride(0), x.stride(1), _ptr(w), _ptr(bias), _ptr(init), _ptr(lengths), _ptr(dy), dy.stride(0),
-            dy.stride(1), _ptr(d_final), _ptr(dx), _ptr(d_init), _ptr(dw), _ptr(dbias), _ptr(scratch),
-            scratch.numel(), K, ctx.silu, _IO[x.dtype], B, T, C, _stream(dev))), "causal_conv1d backward")
+        _run("causal_conv1d backward", L.atlas_causal_conv_backward, dev, x.data_ptr(), x.stride(0), x.stride(1),
+             w.data_ptr(), _ptr(bias), _ptr(init), _ptr(lengths), dy.data_ptr(), dy.stride(0), dy.stride(1),
+             _ptr(d_final), dx.data_ptr(), _ptr(d_init), dw.data_ptr(), _ptr(dbias), scratch.data_ptr(),
+             scratch.numel(), K, ctx.silu, _IO[x.dtype], B, T, C)
         return dx, dw, dbias, d_init, None, None
 
 
@@ -295,7 +304,8 @@ def causal_conv1d(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, acti
     w, bias = _f32(what, "weight", weight, (C, K), dev), _f32(what, "bias", bias, (C,), dev)
     if initial_state is not None:
         _check(what, "initial_state", initial_state, (B, K - 1, C), x.dtype, dev)
-        initial_state = initial_state.contiguous()
+        if not initial_state.is_contiguous():
+            initial_state = initial_state.contiguous()
     lengths = _lengths(what, lengths, B, dev)
     _need_cuda(x, what)
     silu = int(activation == "silu")
@@ -303,6 +313,6 @@ def causal_conv1d(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, acti
         final = x.new_zeros(B, K - 1, C) if initial_state is None else initial_state.clone()
         return torch.empty_like(x, memory_format=torch.contiguous_format), final
     x = _rows(x)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, initial_state)):
+    if _wants_grad(x, w, bias, initial_state):
         return CausalConv1dFn.apply(x, w, bias, initial_state, lengths, silu)
     return _conv_forward(x, w, bias, initial_state, lengths, silu)
