@@ -35,7 +35,8 @@ int launch(bool fwd, ConvArgs a, int64_t B, float* dw, float* dbias, cudaStream_
   const dim3 grid((unsigned)(B * a.ygrid), (unsigned)((a.C + 32 * W - 1) / (32 * W)));
   if (fwd && a.T == 1 && B <= 65535) {
     const dim3 one((unsigned)((a.C + kConvStepThr * W - 1) / (kConvStepThr * W)), (unsigned)B);
-    LAUNCH_T(KID_CONV_STEP, (k_causal_conv_step<K, IO, W>), one, kConvStepThr, 0, st, a);
+    if (a.vec && a.C % W == 0) LAUNCH_T(KID_CONV_STEP, (k_causal_conv_step<K, IO, W, true>), one, kConvStepThr, 0, st, a);
+    else LAUNCH_T(KID_CONV_STEP, (k_causal_conv_step<K, IO, W, false>), one, kConvStepThr, 0, st, a);
     return ATLAS_OK;
   }
   if (fwd) {

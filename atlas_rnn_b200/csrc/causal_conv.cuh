@@ -176,36 +176,50 @@ __global__ void __launch_bounds__(32 * kConvWarps) k_causal_conv_fwd(const ConvA
   for (; t < q.n; ++t) store<IO, W>(y + t * a.C, zeros<IO, W>(), q.nc, q.fast);
 }
 
-// One step (T = 1): a thread reads its channels' K - 1 carried inputs and the new one once, and writes y and the shifted
-// state. grid (channel blocks, batch).
+// One step (T = 1): a thread reads its channels' K - 1 carried inputs and the new one once, all in flight together, and
+// writes y and the shifted state. FAST: whole vectors. grid (channel blocks, batch).
 constexpr int kConvStepThr = 128;
-template <int K, class IO, int W>
+template <int K, class IO, int W, bool FAST>
 __global__ void __launch_bounds__(kConvStepThr) k_causal_conv_step(const ConvArgs a) {
   constexpr int P = W / 2;
   const int64_t b = blockIdx.y, c = ((int64_t)blockIdx.x * kConvStepThr + threadIdx.x) * W;
   if (c >= a.C) return;
   const int nc = a.C - c < W ? (int)(a.C - c) : W;
-  const bool fast = a.vec && nc == W, live = row_len(a.len, (int)b, 1) > 0;
-  Row<IO, W> v[K];
+  auto raw = [&](const IO* p) {
+    if (FAST) return *reinterpret_cast<const Vec<IO, W>*>(p);
+    return ss::load_row<IO, W>(p, 0, nc, 0);
+  };
+  auto put = [&](IO* p, const Vec<IO, W>& r) {
+    if (FAST) *reinterpret_cast<Vec<IO, W>*>(p) = r;
+    else ss::store_row<IO, W>(p, 0, nc, 0, r);
+  };
+  Vec<IO, W> v[K];
 #pragma unroll
   for (int j = 0; j < K - 1; ++j)
-    v[j] = a.init ? load<IO, W>((const IO*)a.init + (b * (K - 1) + j) * a.C + c, nc, fast) : zeros<IO, W>();
-  v[K - 1] = live ? load<IO, W>((const IO*)a.x + b * a.x_sb + c, nc, fast) : zeros<IO, W>();
+    v[j] = a.init ? raw((const IO*)a.init + (b * (K - 1) + j) * a.C + c) : ss::zero_row<IO, W>();
+  v[K - 1] = raw((const IO*)a.x + b * a.x_sb + c);
+  float w[W][K], bias[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const int64_t k = FAST || i < nc ? c + i : c;
+    bias[i] = a.bias ? a.bias[k] : 0.f;
+#pragma unroll
+    for (int j = 0; j < K; ++j) w[i][j] = a.w[k * K + j];
+  }
+  const bool live = row_len(a.len, (int)b, 1) > 0;
   IO* f = (IO*)a.final_state + b * (K - 1) * a.C + c;
 #pragma unroll
-  for (int j = 0; j < K - 1; ++j) store<IO, W>(f + j * a.C, live ? v[j + 1] : v[j], nc, fast);
-  Row<IO, W> o;
+  for (int j = 0; j < K - 1; ++j) put(f + j * a.C, live ? v[j + 1] : v[j]);
+  Vec<IO, W> o;
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    const bool o0 = 2 * i < nc, o1 = 2 * i + 1 < nc;
-    const int64_t k = c + 2 * i;
-    f2 s = pk(a.bias && o0 ? a.bias[k] : 0.f, a.bias && o1 ? a.bias[k + 1] : 0.f);
+    f2 s = pk(bias[2 * i], bias[2 * i + 1]);
 #pragma unroll
-    for (int j = 0; j < K; ++j)
-      s = fma2(pk(o0 ? a.w[k * K + j] : 0.f, o1 ? a.w[(k + 1) * K + j] : 0.f), v[j].v[i], s);
-    o.v[i] = a.silu ? mul2(s, sigmoid_2(s)) : s;
+    for (int j = 0; j < K; ++j) s = fma2(pk(w[2 * i][j], w[2 * i + 1][j]), ld2(&v[j].v[2 * i]), s);
+    if (a.silu) s = mul2(s, sigmoid_2(s));
+    st2(&o.v[2 * i], live ? s : 0);
   }
-  store<IO, W>((IO*)a.y + b * a.C + c, live ? o : zeros<IO, W>(), nc, fast);
+  put((IO*)a.y + b * a.C + c, o);
 }
 
 template <int K, class IO, int W>

@@ -153,15 +153,17 @@ int fwd_t(const AtlasSelScan* a, ScanArgs s, cudaStream_t st) {
 template <class IO, int NP>
 int step_t(const AtlasSelScan* a, ScanArgs s, cudaStream_t st) {
   alignment(a, s, 4);
-  const int vec4 = a->N % 4 == 0 && (uintptr_t)a->A % 16 == 0 && (uintptr_t)a->h0 % 16 == 0 &&
+  const bool v4 = s.vecbc && a->N % 4 == 0 && (uintptr_t)a->A % 16 == 0 && (uintptr_t)a->h0 % 16 == 0 &&
                    (uintptr_t)a->hT % 16 == 0;
   // four rows a thread while that still leaves two waves of threads
   const int64_t per = kStepThr / (NP / 4), gx = (a->D + per - 1) / per, rows = a->B * gx >= 8 * 4 * 148 * 2 ? 4 : 1;
   const int64_t gy = (a->B + rows - 1) / rows;
   if (gx > 0x7fffffff || gy > 65535) return ATLAS_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)gx, (unsigned)gy);
-  if (rows == 4) LAUNCH_T(KID_SSCAN_STEP, (k_sscan_step<IO, NP, 4>), grid, kStepThr, 0, st, s, vec4);
-  else LAUNCH_T(KID_SSCAN_STEP, (k_sscan_step<IO, NP, 1>), grid, kStepThr, 0, st, s, vec4);
+  if (rows == 4 && v4) LAUNCH_T(KID_SSCAN_STEP, (k_sscan_step<IO, NP, 4, true>), grid, kStepThr, 0, st, s);
+  else if (rows == 4) LAUNCH_T(KID_SSCAN_STEP, (k_sscan_step<IO, NP, 4, false>), grid, kStepThr, 0, st, s);
+  else if (v4) LAUNCH_T(KID_SSCAN_STEP, (k_sscan_step<IO, NP, 1, true>), grid, kStepThr, 0, st, s);
+  else LAUNCH_T(KID_SSCAN_STEP, (k_sscan_step<IO, NP, 1, false>), grid, kStepThr, 0, st, s);
   return ATLAS_OK;
 }
 

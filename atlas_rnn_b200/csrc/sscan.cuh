@@ -410,82 +410,74 @@ __global__ void __launch_bounds__(kCarryThr) k_sscan_carry(const ScanArgs a) {
 // traffic) of R batch rows, whose loads are all in flight together; LPC = NP / 4 lanes a channel. A, D and bias are read
 // once for the R rows. grid (channel blocks, row blocks).
 constexpr int kStepThr = 128;
-template <class IO, int NP, int R>
-__global__ void __launch_bounds__(kStepThr) k_sscan_step(const ScanArgs a, int vec4) {
+// V4: 16-byte accesses to A and the states, 4-element ones to B and C (N a multiple of 4)
+template <class IO, int NP, int R, bool V4>
+__global__ void __launch_bounds__(kStepThr) k_sscan_step(const ScanArgs a) {
   constexpr int LPC = NP / 4;
   const int d = blockIdx.x * (kStepThr / LPC) + threadIdx.x / LPC, n4 = threadIdx.x % LPC * 4;
-  const bool on = d < a.Dm;
-  const int dd = on ? d : 0, g = dd / (a.Dm / a.G);
-  const bool v4 = vec4 && n4 < a.N;
-  float A[4] = {0.f, 0.f, 0.f, 0.f}, h[R][4];
-  float dt[R], u[R], z[R];
-  Vec<IO, 4> B[R], C[R];
-  bool live[R];
-  const float* Ap = a.A + (int64_t)dd * a.N + n4;
-  if (v4) {
-    const float4 x = *reinterpret_cast<const float4*>(Ap);
-    A[0] = x.x, A[1] = x.y, A[2] = x.z, A[3] = x.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n4 + i < a.N) A[i] = Ap[i];
-  }
+  const bool on = d < a.Dm && (!V4 || n4 < a.N);
+  const int dd = d < a.Dm ? d : 0, nn = V4 && n4 < a.N ? n4 : 0, g = dd / (a.Dm / a.G);
+  auto four = [&](const float* p) {  // states n4 .. n4 + 3 of a row
+    if (V4) return *reinterpret_cast<const float4*>(p + nn);
+    return make_float4(n4 < a.N ? p[n4] : 0.f, n4 + 1 < a.N ? p[n4 + 1] : 0.f, n4 + 2 < a.N ? p[n4 + 2] : 0.f,
+                       n4 + 3 < a.N ? p[n4 + 3] : 0.f);
+  };
+  auto cols = [&](const IO* p) {
+    if (V4) return *reinterpret_cast<const Vec<IO, 4>*>(p + nn);
+    return load_row<IO, 4>(p, n4, a.N, 0);
+  };
+  // all loads first, of rows that exist (what a dead row holds is dropped below), nothing used before the last is issued
+  const float4 A = four(a.A + (int64_t)dd * a.N);
   const float bias = a.bias ? a.bias[dd] : 0.f, skip = a.D ? a.D[dd] : 0.f;
+  float4 h[R];
+  IO du[R], dd_[R], dz[R];
+  Vec<IO, 4> B[R], C[R];
+  int len[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int64_t b = (int64_t)blockIdx.y * R + r;
-    const bool row = on && b < a.Bsz;
-    live[r] = row && row_len(a.len, (int)(row ? b : 0), 1) > 0;
-    const int64_t at = (row ? b * a.Dm + d : 0) * a.N + n4;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[r][i] = 0.f;
-    if (row && a.h0) {
-      if (v4) {
-        const float4 x = *reinterpret_cast<const float4*>(a.h0 + at);
-        h[r][0] = x.x, h[r][1] = x.y, h[r][2] = x.z, h[r][3] = x.w;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (n4 + i < a.N) h[r][i] = a.h0[at + i];
-      }
-    }
-    u[r] = dt[r] = z[r] = 0.f;
-    B[r] = C[r] = zero_row<IO, 4>();
-    if (live[r]) {
-      u[r] = to_f(((const IO*)a.u)[b * a.u_sb + d]);
-      dt[r] = to_f(((const IO*)a.delta)[b * a.d_sb + d]);
-      if (a.z) z[r] = to_f(((const IO*)a.z)[b * a.z_sb + d]);
-      B[r] = load_row<IO, 4>((const IO*)a.Bm + b * a.B_sb + g * a.B_sg, n4, a.N, a.vecbc);
-      C[r] = load_row<IO, 4>((const IO*)a.Cm + b * a.C_sb + g * a.C_sg, n4, a.N, a.vecbc);
-    }
+    const int64_t b = (int64_t)blockIdx.y * R + r < a.Bsz ? (int64_t)blockIdx.y * R + r : 0;
+    h[r] = a.h0 ? four(a.h0 + (b * a.Dm + dd) * a.N) : make_float4(0.f, 0.f, 0.f, 0.f);
+    du[r] = ((const IO*)a.u)[b * a.u_sb + dd];
+    dd_[r] = ((const IO*)a.delta)[b * a.d_sb + dd];
+    dz[r] = ((const IO*)(a.z ? a.z : a.u))[a.z ? b * a.z_sb + dd : 0];
+    B[r] = cols((const IO*)a.Bm + b * a.B_sb + g * a.B_sg);
+    C[r] = cols((const IO*)a.Cm + b * a.C_sb + g * a.C_sg);
+    len[r] = a.len ? a.len[b] : 1;
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int64_t b = (int64_t)blockIdx.y * R + r;
-    float x = dt[r] + bias, y = 0.f;
+    const bool live = len[r] > 0;
+    float hv[4] = {h[r].x, h[r].y, h[r].z, h[r].w}, y = 0.f;
+    const float Av[4] = {A.x, A.y, A.z, A.w}, u = live ? to_f(du[r]) : 0.f;
+    float x = to_f(dd_[r]) + bias;
     if (a.softplus) x = softplus(x);
-    if (!live[r]) x = 0.f;
-    const float xl = x * kLog2e, du = x * u[r];
+    if (!live) x = 0.f;
+    const float xl = x * kLog2e, xu = x * u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      h[r][i] = fmaf(ex2(A[i] * xl), h[r][i], du * to_f(B[r].v[i]));
-      y = fmaf(to_f(C[r].v[i]), h[r][i], y);
+      const float Bv = live ? to_f(B[r].v[i]) : 0.f, Cv = live ? to_f(C[r].v[i]) : 0.f;
+      hv[i] = fmaf(ex2(Av[i] * xl), hv[i], xu * Bv);
+      if (V4 ? on : n4 + i < a.N) y = fmaf(Cv, hv[i], y);
     }
 #pragma unroll
     for (int o = LPC / 2; o >= 1; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (!on || b >= a.Bsz) continue;
+    if (d >= a.Dm || b >= a.Bsz) continue;
     float* ho = a.hT + (b * a.Dm + d) * a.N + n4;
-    if (v4) {
-      *reinterpret_cast<float4*>(ho) = make_float4(h[r][0], h[r][1], h[r][2], h[r][3]);
+    if (V4) {
+      if (on) *reinterpret_cast<float4*>(ho) = make_float4(hv[0], hv[1], hv[2], hv[3]);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (n4 + i < a.N) ho[i] = h[r][i];
+        if (n4 + i < a.N) ho[i] = hv[i];
     }
     if (n4 == 0) {
-      y = fmaf(skip, u[r], y);
-      if (a.z) y *= z[r] * sigmoid(z[r]);
-      from_f(((IO*)a.out)[b * a.Dm + d], live[r] ? y : 0.f);
+      y = fmaf(skip, u, y);
+      if (a.z) {
+        const float zz = to_f(dz[r]);
+        y *= zz * sigmoid(zz);
+      }
+      from_f(((IO*)a.out)[b * a.Dm + d], live ? y : 0.f);
     }
   }
 }
