@@ -24,6 +24,7 @@ from torch import Tensor, cat, nn
 from torch.nn import Module, ModuleList
 
 from .rnn_memory import OmegaRNNMemoryCell, RNNMemoryCell, RNNMemState, exists
+from .sampling import sample_tokens
 
 
 def log(t: Tensor, eps: float = 1e-20) -> Tensor:
@@ -134,9 +135,11 @@ class RNNMemoryTransformer(Module):
 
     @torch.no_grad()
     def generate(self, prompt: Tensor, max_length: int = 100, temperature: float = 1.0, min_p: float = 0.1,
-                 use_cache: bool = True) -> Tensor:
+                 use_cache: bool = True, top_k: int = 0, top_p: float = 1.0) -> Tensor:
         """Autoregressive sampling (rnn_transformer.py:864-904). With the cache each new
-        token is one T = 1 call per layer, which runs the single-token decode kernel."""
+        token is one T = 1 call per layer, which runs the single-token decode kernel. With
+        top_k or top_p set, the filters (these two before min_p) and the draw are one
+        ``sample_tokens`` kernel per token."""
         self.eval()
         full = prompt.clone()
         x, states = prompt, None
@@ -145,8 +148,14 @@ class RNNMemoryTransformer(Module):
                 logits, states, _ = self(x, mem_states=states, return_cache=True)
             else:
                 logits = self(full)
-            logits = min_p_filter(logits[:, -1:], min_p=min_p)
-            nxt = gumbel_sample(logits, temperature=temperature).squeeze(-1)
+            if top_k > 0 or top_p < 1.0:
+                last = logits[:, -1:]
+                last = last if last.dtype == torch.bfloat16 else last.float()
+                nxt = sample_tokens(last, torch.rand(last.shape, device=last.device), temperature=temperature,
+                                    top_k=top_k, top_p=top_p, min_p=min_p)
+            else:
+                logits = min_p_filter(logits[:, -1:], min_p=min_p)
+                nxt = gumbel_sample(logits, temperature=temperature).squeeze(-1)
             full = cat([full, nxt], dim=-1)
             x = nxt if use_cache else full
         return full

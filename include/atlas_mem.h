@@ -463,6 +463,28 @@ int atlas_causal_conv_backward(const void* x, int64_t x_sb, int64_t x_st, const 
                                size_t scratch_bytes, int K, int silu, int dtype_io, int64_t B, int64_t T, int64_t C,
                                void* stream);
 
+/* Token sampling with given uniforms (the filters and the draw of generate, rnn_transformer.py:42-59, with top-k and
+ * top-p beside its min-p). Per row of logits [rows, V] (fp32 or bf16, rows `stride` elements apart; NaN counts as
+ * -inf), in the order of descending logit, ties by lowest index:
+ *   top-k: the first top_k tokens (<= 0 or >= V: all);
+ *   top-p: of those, the tokens with less than top_p of their mass exp(logit) before them (the first always; >= 1: all);
+ *   min-p: of those, the tokens with at least min_p times the first one's probability (the first always);
+ *   out = argmax over the kept of logit / temperature - log(-log u), u from noise [rows, V] fp32 in [0, 1], clamped as
+ *   gumbel_noise clamps (1e-20); temperature <= 0: the first token. A row without any logit above -inf gives 0.
+ * Each setting is one value, or an array of one per row where its _row pointer is given. */
+typedef struct AtlasSample {
+  const void* logits;
+  const float* noise;
+  int64_t* out;
+  int64_t rows, V, stride, noise_stride;
+  double temperature, top_p, min_p;
+  int64_t top_k;
+  const float *temperature_row, *top_p_row, *min_p_row;
+  const int32_t* top_k_row;
+  int32_t dtype;
+} AtlasSample;
+int atlas_sample_tokens(const AtlasSample* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -103,3 +103,50 @@ def test_native_calls_refuse_bad_arguments(native_lib):
     assert native_lib.atlas_sscan_forward(_SCAN.pack(*fields()), None) == 1  # null operands
     assert native_lib.atlas_causal_conv_scratch(1, 8, 4, 9) == 0
     assert native_lib.atlas_causal_conv_forward(*([None, 0, 0] + [None] * 6 + [4, 1, 0, 1, 8, 4, None])) == 1
+
+
+def test_sample_argument_record_matches_header():
+    from atlas_rnn_b200.sampling import _SAMPLE
+    prog = '#include <stdio.h>\n#include <stddef.h>\n#include "atlas_mem.h"\nint main(void) {\n' \
+           'printf("%zu %zu %zu\\n", sizeof(AtlasSample), offsetof(AtlasSample, top_k), offsetof(AtlasSample, dtype));\n' \
+           'return 0; }\n'
+    with tempfile.TemporaryDirectory() as td:
+        c, exe = os.path.join(td, "t.c"), os.path.join(td, "t")
+        open(c, "w").write(prog)
+        subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), c, "-o", exe], check=True)
+        size, at_k, at_dtype = map(int, subprocess.run([exe], capture_output=True, text=True).stdout.split())
+    assert _SAMPLE.size == size
+    raw = _SAMPLE.pack(0, 0, 0, 0, 0, 0, 0, 0.0, 0.0, 0.0, 0x1122, 0, 0, 0, 0, 0x3344)
+    assert int.from_bytes(raw[at_k:at_k + 8], "little") == 0x1122
+    assert int.from_bytes(raw[at_dtype:at_dtype + 4], "little") == 0x3344
+
+
+@pytest.mark.parametrize("change, error", [
+    (dict(logits=torch.zeros(2, 5, dtype=torch.float16)), TypeError),
+    (dict(logits=torch.zeros(())), ValueError),
+    (dict(logits=torch.zeros(2, 0)), ValueError),
+    (dict(noise=torch.zeros(2, 4)), ValueError),
+    (dict(noise=torch.zeros(2, 5, dtype=torch.float64)), TypeError),
+    (dict(temperature=-0.1), ValueError),
+    (dict(temperature=float("nan")), ValueError),
+    (dict(top_k=-1), ValueError),
+    (dict(top_p=1.1), ValueError),
+    (dict(top_p=-0.1), ValueError),
+    (dict(min_p=2.0), ValueError),
+    (dict(top_k=torch.zeros(2)), TypeError),
+    (dict(top_p=torch.zeros(2, dtype=torch.int32)), TypeError),
+    (dict(temperature=torch.zeros(3)), ValueError),
+    (dict(), RuntimeError),
+])
+def test_sample_refusals(change, error):
+    args = dict(logits=torch.zeros(2, 5), noise=torch.zeros(2, 5))
+    with pytest.raises(error):
+        A.sample_tokens(**{**args, **change})
+
+
+def test_native_sample_refuses_bad_arguments(native_lib):
+    from atlas_rnn_b200.sampling import _SAMPLE
+    assert native_lib.atlas_sample_tokens(None, None) == 1
+    for rows, V, dt in ((0, 5, 0), (1, 0, 0), (1, 5, 7), (1, 1 << 31, 0)):
+        assert native_lib.atlas_sample_tokens(_SAMPLE.pack(16, 16, 16, rows, V, 5, 5, 1.0, 1.0, 0.0, 0, 0, 0, 0, 0, dt), None) == 1
+    assert native_lib.atlas_sample_tokens(_SAMPLE.pack(0, 16, 16, 1, 5, 5, 5, 1.0, 1.0, 0.0, 0, 0, 0, 0, 0, 0), None) == 1
