@@ -14,11 +14,12 @@ from .omega_store import omega_store_update
 from .affine_scan import affine_associative_scan
 from .selective_scan import causal_conv1d, selective_scan
 from .sampling import sample_tokens
+from .distill import distill_loss
 from .rnn_memory import (RNNMemState, state_detach, PolynomialFeatureMap, MultiheadRMSNorm,
                          RNNMemoryCell, OmegaRNNMemoryCell, RNNMemory, OmegaRNNMemory)
 from .rnn_transformer import LMMBlock, LongTermMemoryModel, RNNMemoryTransformer
 
 __all__ = ["memory_recurrence", "MemoryRecurrenceFn", "check_device_status", "AssocScan", "assoc_scan", "omega_store_update", "affine_associative_scan",
-           "causal_conv1d", "selective_scan", "sample_tokens", "RNNMemState", "state_detach",
+           "causal_conv1d", "selective_scan", "sample_tokens", "distill_loss", "RNNMemState", "state_detach",
            "PolynomialFeatureMap", "MultiheadRMSNorm", "RNNMemoryCell", "OmegaRNNMemoryCell",
            "RNNMemory", "OmegaRNNMemory", "LMMBlock", "LongTermMemoryModel", "RNNMemoryTransformer"]

@@ -121,6 +121,9 @@ def lib():
         L.atlas_sscan_forward.restype = ctypes.c_int
         L.atlas_sscan_backward.argtypes = [ctypes.c_char_p, _vp]
         L.atlas_sscan_backward.restype = ctypes.c_int
+        for name in ("atlas_distill_forward", "atlas_distill_backward"):
+            getattr(L, name).argtypes = [ctypes.c_char_p, _vp]
+            getattr(L, name).restype = ctypes.c_int
         L.atlas_sample_tokens.argtypes = [ctypes.c_char_p, _vp]
         L.atlas_sample_tokens.restype = ctypes.c_int
         L.atlas_causal_conv_forward.argtypes = [_vp, i64, i64] + [_vp] * 6 + [ci] * 3 + [i64] * 3 + [_vp]

@@ -23,6 +23,7 @@ import torch.nn.functional as F
 from torch import Tensor, cat, nn
 from torch.nn import Module, ModuleList
 
+from .distill import distill_loss
 from .rnn_memory import OmegaRNNMemoryCell, RNNMemoryCell, RNNMemState, exists
 from .sampling import sample_tokens
 
@@ -117,7 +118,13 @@ class RNNMemoryTransformer(Module):
         nn.init.normal_(self.to_logits.weight, std=0.02)
 
     def forward(self, x: Tensor, return_loss: bool = False, mem_states=None, attn_caches=None,
-                return_cache: bool = False):
+                return_cache: bool = False, teacher=None, distill_weight: float = 0.5,
+                distill_temperature: float = 1.0):
+        """Logits, or with ``return_loss`` the next-token loss. teacher: (values, indices) [b, n - 1, K], a teacher's
+        top logits for the n - 1 predicted positions; the loss is then
+        (1 - distill_weight) cross-entropy + distill_weight ``distill_loss`` at distill_temperature."""
+        if exists(teacher) and not return_loss:
+            raise ValueError("teacher logits are used for the loss: pass return_loss=True")
         if return_loss:
             x, labels = x[:, :-1], x[:, 1:]
         h = self.embed_norm(self.embed(x))
@@ -130,6 +137,10 @@ class RNNMemoryTransformer(Module):
         caches = [None] * self.depth
         if return_loss:
             loss = F.cross_entropy(logits.view(-1, self.num_tokens), labels.reshape(-1))
+            if exists(teacher):
+                student = logits if logits.dtype == torch.bfloat16 else logits.float()
+                distilled = distill_loss(student, *teacher, temperature=distill_temperature)
+                loss = (1 - distill_weight) * loss + distill_weight * distilled
             return (loss, logits, new_states, caches) if return_cache else loss
         return (logits, new_states, caches) if return_cache else logits
 

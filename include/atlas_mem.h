@@ -485,6 +485,27 @@ typedef struct AtlasSample {
 } AtlasSample;
 int atlas_sample_tokens(const AtlasSample* a, void* stream);
 
+/* Distillation from a teacher's top logits (beside the language model's cross-entropy, rnn_transformer.py:852-860). Per row
+ * of student logits x [rows, V] (fp32 or bf16, rows `stride` elements apart), with the teacher's K entries (values fp32,
+ * indices int64 [rows, K]; absent where the index is outside 0 .. V-1 or the value is -inf or NaN):
+ *   p = softmax(values / temperature) over the entries, q = softmax(x / temperature),
+ *   loss = temperature^2 sum_k p_k (log p_k - log q[index_k]), 0 for a row without entries (valid = 0, else 1);
+ *   dlogits [rows, V] = dloss temperature (q - sum of p at the token). Tokens may repeat. 1 <= K <= 1024.
+ * stats [rows, 4] fp32 (16-byte aligned) is written by the forward and read by the backward. */
+typedef struct AtlasDistill {
+  const void* logits;
+  const float* values;
+  const int64_t* indices;
+  float *loss, *valid, *stats;
+  const float* dloss;
+  void* dlogits;
+  int64_t rows, V, K, stride;
+  float temperature;
+  int32_t dtype;
+} AtlasDistill;
+int atlas_distill_forward(const AtlasDistill* a, void* stream);
+int atlas_distill_backward(const AtlasDistill* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -150,3 +150,57 @@ def test_native_sample_refuses_bad_arguments(native_lib):
     for rows, V, dt in ((0, 5, 0), (1, 0, 0), (1, 5, 7), (1, 1 << 31, 0)):
         assert native_lib.atlas_sample_tokens(_SAMPLE.pack(16, 16, 16, rows, V, 5, 5, 1.0, 1.0, 0.0, 0, 0, 0, 0, 0, dt), None) == 1
     assert native_lib.atlas_sample_tokens(_SAMPLE.pack(0, 16, 16, 1, 5, 5, 5, 1.0, 1.0, 0.0, 0, 0, 0, 0, 0, 0), None) == 1
+
+
+def test_distill_argument_record_matches_header():
+    from atlas_rnn_b200.distill import _DISTILL
+    prog = '#include <stdio.h>\n#include <stddef.h>\n#include "atlas_mem.h"\nint main(void) {\n' \
+           'printf("%zu %zu %zu\\n", sizeof(AtlasDistill), offsetof(AtlasDistill, rows), offsetof(AtlasDistill, dtype));\n' \
+           'return 0; }\n'
+    with tempfile.TemporaryDirectory() as td:
+        c, exe = os.path.join(td, "t.c"), os.path.join(td, "t")
+        open(c, "w").write(prog)
+        subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), c, "-o", exe], check=True)
+        size, at_rows, at_dtype = map(int, subprocess.run([exe], capture_output=True, text=True).stdout.split())
+    assert _DISTILL.size == size
+    raw = _DISTILL.pack(*[0] * 8, 0x1122, 0, 0, 0, 0.0, 0x3344)
+    assert int.from_bytes(raw[at_rows:at_rows + 8], "little") == 0x1122
+    assert int.from_bytes(raw[at_dtype:at_dtype + 4], "little") == 0x3344
+
+
+@pytest.mark.parametrize("change, error", [
+    (dict(logits=torch.zeros(2, 5, dtype=torch.float16)), TypeError),
+    (dict(logits=torch.zeros(2, 0)), ValueError),
+    (dict(teacher_values=torch.zeros(2, 0)), ValueError),
+    (dict(teacher_values=torch.zeros(2, 1025), teacher_indices=torch.zeros(2, 1025, dtype=torch.int64)), ValueError),
+    (dict(teacher_values=torch.zeros(2, 3, dtype=torch.int32)), TypeError),
+    (dict(teacher_indices=torch.zeros(2, 3)), TypeError),
+    (dict(teacher_indices=torch.zeros(2, 4, dtype=torch.int64)), ValueError),
+    (dict(teacher_values=torch.zeros(3, 3)), ValueError),
+    (dict(temperature=0.0), ValueError),
+    (dict(temperature=float("inf")), ValueError),
+    (dict(reduction="batchmean"), ValueError),
+    (dict(), RuntimeError),
+])
+def test_distill_refusals(change, error):
+    args = dict(logits=torch.zeros(2, 5), teacher_values=torch.zeros(2, 3),
+                teacher_indices=torch.zeros(2, 3, dtype=torch.int64))
+    with pytest.raises(error):
+        A.distill_loss(**{**args, **change})
+
+
+def test_teacher_without_a_loss_is_refused():
+    m = A.RNNMemoryTransformer(num_tokens=8, dim=8, depth=1, heads=1, dim_head=8)
+    with pytest.raises(ValueError):
+        m(torch.zeros(1, 3, dtype=torch.int64), teacher=(torch.zeros(1, 2, 1), torch.zeros(1, 2, 1, dtype=torch.int64)))
+
+
+def test_native_distill_refuses_bad_arguments(native_lib):
+    from atlas_rnn_b200.distill import _DISTILL
+    assert native_lib.atlas_distill_forward(None, None) == 1 and native_lib.atlas_distill_backward(None, None) == 1
+    ok = dict(rows=1, V=5, K=2, t=1.0, dt=0)
+    for bad in (dict(rows=0), dict(V=0), dict(K=0), dict(K=1025), dict(t=0.0), dict(t=float("nan")), dict(dt=3)):
+        f = {**ok, **bad}
+        raw = _DISTILL.pack(*[16] * 8, f["rows"], f["V"], f["K"], 5, f["t"], f["dt"])
+        assert native_lib.atlas_distill_forward(raw, None) == 1 and native_lib.atlas_distill_backward(raw, None) == 1, bad
+    assert native_lib.atlas_distill_forward(_DISTILL.pack(*[0] * 8, 1, 5, 2, 5, 1.0, 0), None) == 1
