@@ -28,7 +28,7 @@ struct DistillArgs {
   float* stats;            // [rows, 4]: m and log2 s of the student; maximum and sum of the teacher (0: no entries)
   const float* dloss;
   void* dlogits;  // [rows, V]
-  int V, K, split, vec;
+  int V, K, split;
   float tau;
 };
 
@@ -40,6 +40,22 @@ __device__ __forceinline__ T warp_reduce(T v, F f) {
 }
 __device__ __forceinline__ float fmax_op(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ float add_op(float a, float b) { return a + b; }
+
+// Elements before the first 16-byte boundary of a row (all n of them if it lies behind).
+template <class IO>
+__device__ __forceinline__ int head_of(const IO* p, int n) {
+  const int h = (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(IO);
+  return h < n ? h : n;
+}
+// Largest of a vector's elements (NaN is none).
+__device__ __forceinline__ float vec_max(const ss::Vec<float, 4>& r) {
+  return fmaxf(fmaxf(r.v[0], r.v[1]), fmaxf(r.v[2], r.v[3]));
+}
+__device__ __forceinline__ float vec_max(const ss::Vec<__nv_bfloat16, 8>& r) {
+  const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(r.v);
+  const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
 
 // Value and token of entry k, -inf where it is absent.
 __device__ __forceinline__ float entry(const DistillArgs& a, int64_t row, int k, int64_t& token) {
@@ -73,57 +89,51 @@ __global__ void __launch_bounds__(NT) k_distill_fwd(const DistillArgs a) {
       m = top;
     }
   };
-  int done = 0;
-  if (a.vec) {
-    const int nv = n / E;
-    int v = tid;
-    for (; v + (U - 1) * NT < nv; v += U * NT) {
-      ss::Vec<IO, E> r[U];
+  // the first warp's first entries, their logits on the way while the row streams by
+  float v0[2], x0[2];
 #pragma unroll
-      for (int i = 0; i < U; ++i) r[i] = *reinterpret_cast<const ss::Vec<IO, E>*>(x + lo + (v + i * NT) * E);
-      float top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < U; ++i)
-#pragma unroll
-        for (int e = 0; e < E; ++e) top = fmaxf(top, ss::to_f(r[i].v[e]));
-      raise(top);
-      if (m > -INFINITY) {
-        float p[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-#pragma unroll
-          for (int e = 0; e < E; ++e) p[e & 1] += ss::ex2((ss::to_f(r[i].v[e]) - m) * c);
-        s += p[0] + p[1];
-      }
-    }
-    for (; v < nv; v += NT) {
-      const ss::Vec<IO, E> r = *reinterpret_cast<const ss::Vec<IO, E>*>(x + lo + v * E);
-      float top = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < E; ++e) top = fmaxf(top, ss::to_f(r.v[e]));
-      raise(top);
-      if (m > -INFINITY) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) s += ss::ex2((ss::to_f(r.v[e]) - m) * c);
-      }
-    }
-    done = nv * E;
+  for (int i = 0; i < 2; ++i) {
+    int64_t t0 = -1;
+    v0[i] = rank == 0 && warp == 0 && lane + 32 * i < a.K ? entry(a, row, lane + 32 * i, t0) : -INFINITY;
+    x0[i] = v0[i] > -INFINITY ? ss::to_f(x[t0]) : 0.f;
   }
-  for (int i = done + tid; i < n; i += NT) {
-    const float v = ss::to_f(x[lo + i]);
+  const IO* xl = x + lo;
+  const int head = head_of(xl, n), nv = (n - head) / E;
+  for (int v = tid; v < nv; v += U * NT) {
+    ss::Vec<IO, E> r[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (v + i * NT < nv) r[i] = *reinterpret_cast<const ss::Vec<IO, E>*>(xl + head + (v + i * NT) * E);
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (v + i * NT < nv) top = fmaxf(top, vec_max(r[i]));
+    raise(top);
+    // with nothing above -inf so far only a NaN, which is no maximum, may reach the sum: 2^(c (-inf - 0)) is 0
+    const ss::f2 base = ss::both(m > -INFINITY ? -m : 0.f), c2 = ss::both(c);
+    ss::f2 p = 0;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (v + i * NT < nv) {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) p = ss::add2(p, ss::ex2_2(ss::mul2(ss::add2(ss::ld2(&r[i].v[e]), base), c2)));
+      }
+    const float2 q = ss::up(p);
+    s += q.x + q.y;
+  }
+  for (int i = tid; i < n - nv * E; i += NT) {  // before and behind the vectors
+    const float v = ss::to_f(xl[i < head ? i : i + nv * E]);
     raise(v);
-    if (m > -INFINITY) s += ss::ex2((v - m) * c);
-    else if (v != v) s = v;  // a NaN is no maximum: it has to reach the sum
+    s += ss::ex2((m > -INFINITY ? v - m : v) * c);
   }
   // over the block, then the cluster; sums of empty parts weigh 2^-inf = 0
   auto join = [&](float m0, float s0, float m1) { return m0 > -INFINITY ? s0 * ss::ex2((m0 - m1) * c) : s0; };
-  float wm = warp_reduce(m, fmax_op);
-  float ws = warp_reduce(join(m, s, wm), add_op);
+  const float wm = warp_reduce(m, fmax_op), ws = warp_reduce(join(m, s, wm), add_op);
   if (lane == 0) s_m[warp] = wm, s_s[warp] = ws;
   __syncthreads();
-  float bm = s_m[0], bs = 0.f;
-  for (int i = 1; i < NW; ++i) bm = fmaxf(bm, s_m[i]);
-  for (int i = 0; i < NW; ++i) bs += join(s_m[i], s_s[i], bm);
+  if (warp != 0 && C == 1) return;  // the first warp finishes the row: no further block barriers
+  const float lm = lane < NW ? s_m[lane] : -INFINITY, lsum = lane < NW ? s_s[lane] : 0.f;
+  float bm = warp_reduce(lm, fmax_op), bs = warp_reduce(join(lm, lsum, bm), add_op);
   if (C > 1) {
     cluster.barrier_wait();
     if (tid == 0) {
@@ -131,41 +141,38 @@ __global__ void __launch_bounds__(NT) k_distill_fwd(const DistillArgs a) {
       *cluster.map_shared_rank(&s_cs[rank], 0) = bs;
     }
     cluster.sync();
-    if (rank != 0) return;
-    bm = s_cm[0], bs = 0.f;
-    for (int i = 1; i < C; ++i) bm = fmaxf(bm, s_cm[i]);
-    for (int i = 0; i < C; ++i) bs += join(s_cm[i], s_cs[i], bm);
+    if (rank != 0 || warp != 0) return;
+    const float cm = lane < C ? s_cm[lane] : -INFINITY, cs = lane < C ? s_cs[lane] : 0.f;
+    bm = warp_reduce(cm, fmax_op), bs = warp_reduce(join(cm, cs, bm), add_op);
   }
   const float ls = log2f(bs);
   // the teacher: maximum, sum, loss
-  float top = -INFINITY;
-  for (int k = tid; k < a.K; k += NT) {
+  float top = fmaxf(v0[0], v0[1]);
+  for (int k = lane + 64; k < a.K; k += 32) {
     int64_t t;
     top = fmaxf(top, entry(a, row, k, t));
   }
   top = warp_reduce(top, fmax_op);
-  __syncthreads();
-  if (lane == 0) s_m[warp] = top;
-  __syncthreads();
-  for (int i = 0; i < NW; ++i) top = fmaxf(top, s_m[i]);
   float sum = 0.f, dot = 0.f;  // dot: sum of weight x (log2 weight - log2 q)
-  for (int k = tid; k < a.K; k += NT) {
-    int64_t t;
-    const float v = entry(a, row, k, t), w = weight(v, top, c);
+  auto count = [&](float v, float xt) {
+    const float w = weight(v, top, c);
     if (w > 0.f) {
       const float lw = v == top ? 0.f : (v - top) * c;
       sum += w;
-      dot += w * (lw - ((ss::to_f(x[t]) - bm) * c - ls));
+      dot += w * (lw - ((xt - bm) * c - ls));
     }
+  };
+  count(v0[0], x0[0]);
+  count(v0[1], x0[1]);
+#pragma unroll 2
+  for (int k = lane + 64; k < a.K; k += 32) {
+    int64_t t;
+    const float v = entry(a, row, k, t);
+    if (v > -INFINITY) count(v, ss::to_f(x[t]));
   }
   sum = warp_reduce(sum, add_op);
   dot = warp_reduce(dot, add_op);
-  __syncthreads();
-  if (lane == 0) s_m[warp] = sum, s_s[warp] = dot;
-  __syncthreads();
-  if (tid == 0) {
-    sum = dot = 0.f;
-    for (int i = 0; i < NW; ++i) sum += s_m[i], dot += s_s[i];
+  if (lane == 0) {
     const bool some = top > -INFINITY;
     a.loss[row] = some ? a.tau * a.tau * 0.6931471805599453f * (dot / sum - log2f(sum)) : 0.f;
     a.valid[row] = some ? 1.f : 0.f;
@@ -194,28 +201,32 @@ __global__ void __launch_bounds__(NT) k_distill_bwd(const DistillArgs a, int C) 
     s_p[k] = v > -INFINITY ? weight(v, st.z, c) / st.w : 0.f;
   }
   auto grad = [&](float v) { return some ? g * ss::ex2(fmaf(v - st.x, c, -st.y)) : 0.f; };
-  int done = 0;
-  if (a.vec) {
-    const int nv = n / E;
+  const IO* xl = x + lo;
+  IO* ol = o + lo;
+  // vectors where both rows reach 16 bytes at the same element
+  const bool both = (((uintptr_t)xl ^ (uintptr_t)ol) & 15) == 0;
+  const int head = both ? head_of(xl, n) : 0, nv = both ? (n - head) / E : 0;
 #pragma unroll 1
-    for (int v = tid; v < nv; v += U * NT) {
-      ss::Vec<IO, E> r[U];
+  for (int v = tid; v < nv; v += U * NT) {
+    ss::Vec<IO, E> r[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (v + i * NT < nv) r[i] = *reinterpret_cast<const ss::Vec<IO, E>*>(x + lo + (v + i * NT) * E);
+    for (int i = 0; i < U; ++i)
+      if (v + i * NT < nv) r[i] = *reinterpret_cast<const ss::Vec<IO, E>*>(xl + head + (v + i * NT) * E);
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (v + i * NT < nv) {
-          ss::Vec<IO, E> y;
+    for (int i = 0; i < U; ++i)
+      if (v + i * NT < nv) {
+        ss::Vec<IO, E> y;
 #pragma unroll
-          for (int e = 0; e < E; e += 2)
-            ss::st2(&y.v[e], ss::pk(grad(ss::to_f(r[i].v[e])), grad(ss::to_f(r[i].v[e + 1]))));
-          *reinterpret_cast<ss::Vec<IO, E>*>(o + lo + (v + i * NT) * E) = y;
-        }
-    }
-    done = nv * E;
+        for (int e = 0; e < E; e += 2)
+          ss::st2(&y.v[e], ss::pk(grad(ss::to_f(r[i].v[e])), grad(ss::to_f(r[i].v[e + 1]))));
+        *reinterpret_cast<ss::Vec<IO, E>*>(ol + head + (v + i * NT) * E) = y;
+      }
   }
-  for (int i = done + tid; i < n; i += NT) ss::from_f(o[lo + i], grad(ss::to_f(x[lo + i])));
+#pragma unroll 4
+  for (int i = tid; i < n - nv * E; i += NT) {
+    const int at = i < head ? i : i + nv * E;
+    ss::from_f(ol[at], grad(ss::to_f(xl[at])));
+  }
   __syncthreads();  // the entries' own values go over those above; equal tokens write the same sum
   for (int k = tid; k < a.K; k += NT) {
     const int t = s_t[k];

@@ -72,8 +72,6 @@ extern "C" int atlas_sample_tokens(const AtlasSample* p, void* stream) {
   a.temperature = p->temperature, a.top_p = p->top_p, a.min_p = p->min_p, a.top_k = p->top_k;
   a.temperature_row = p->temperature_row, a.top_p_row = p->top_p_row, a.min_p_row = p->min_p_row;
   a.top_k_row = p->top_k_row;
-  const int size = p->dtype == ATLAS_BF16 ? 2 : 4, E = 16 / size;
-  a.vec = (uintptr_t)p->logits % 16 == 0 && p->stride % E == 0;
   cudaStream_t st = (cudaStream_t)stream;
   // long rows: 512 threads a CTA
   const bool wide = p->V > 4096;

@@ -41,7 +41,7 @@ struct SampleArgs {
   const float* noise;  // [rows, V], `noise_stride` apart
   int64_t stride, noise_stride;
   int64_t* out;
-  int V, split, vec;  // split: tokens per CTA, a multiple of 16
+  int V, split;  // split: tokens per CTA, a multiple of 16
   // one setting for all rows, or one per row where the pointer is given
   double temperature, top_p, min_p;
   int64_t top_k;
@@ -157,26 +157,30 @@ struct Row {
   };
   const IO* p;
   Ring* ring;
-  int lo, n, vec, tid;
+  int lo, n, tid;
   // f(logits, indices) over the CTA's tokens in batches; a logit as it is in memory, NaN in the places that are none. Each
   // thread feeds itself through its own slots of the ring.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
     float l[kBatch];
     int id[kBatch];
-    const int nv = vec ? n / E : 0;
+    // vectors from the row's first 16-byte boundary on
+    const IO* q0 = p + lo;
+    int head = (int)((16 - ((uintptr_t)q0 & 15)) & 15) / (int)sizeof(IO);
+    head = head < n ? head : n;
+    const int nv = (n - head) / E;
     int next = tid, put = 0, get = 0;
     auto load = [&] {
 #pragma unroll
       for (int q = 0; q < U; ++q)
-        if (next + q * NT < nv) ss::cp_piece<16>(&ring->v[put][q][tid], p + lo + (next + q * NT) * E, 16);
+        if (next + q * NT < nv) ss::cp_piece<16>(&ring->v[put][q][tid], q0 + head + (next + q * NT) * E, 16);
       ss::cp_commit();
       next += U * NT;
       put = put == kAhead ? 0 : put + 1;
     };
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) load();
-    int v = tid, k = nv * E + tid;  // next vector, next single token behind the vectors
+    int v = tid, k = tid;  // next vector, next single token beside the vectors
 #pragma unroll 1
     for (;;) {
       if (v < nv) {
@@ -187,18 +191,19 @@ struct Row {
           const ss::Vec<IO, E> x = *reinterpret_cast<const ss::Vec<IO, E>*>(&raw);
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            id[q * E + e] = lo + (v + q * NT) * E + e;
+            id[q * E + e] = lo + head + (v + q * NT) * E + e;
             l[q * E + e] = v + q * NT < nv ? ss::to_f(x.v[e]) : NAN;
           }
         }
         v += U * NT;
         get = get == kAhead ? 0 : get + 1;
         load();  // into the slot of the batch before this one
-      } else if (k < n) {
+      } else if (k < n - nv * E) {
 #pragma unroll
         for (int e = 0; e < kBatch; ++e) {
-          id[e] = lo + k + e * NT;
-          l[e] = k + e * NT < n ? ss::to_f(p[id[e]]) : NAN;
+          const int at = k + e * NT;
+          id[e] = lo + (at < head ? at : at + nv * E);
+          l[e] = at < n - nv * E ? ss::to_f(p[id[e]]) : NAN;
         }
         k += kBatch * NT;
       } else {
@@ -227,7 +232,7 @@ __global__ void __launch_bounds__(NT) k_sample(const SampleArgs a) {
   r.p = (const IO*)a.logits + row * a.stride;
   r.lo = rank * a.split;
   r.n = a.V - r.lo < a.split ? (a.V - r.lo < 0 ? 0 : a.V - r.lo) : a.split;
-  r.vec = a.vec, r.tid = tid;
+  r.tid = tid;
   r.ring = reinterpret_cast<typename Row<IO, NT>::Ring*>(sm_raw + sizeof(Smem));
   const float* noise = a.noise + row * a.noise_stride;
 
