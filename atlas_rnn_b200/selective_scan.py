@@ -11,6 +11,7 @@ No reference counterpart.
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 
 import torch
@@ -93,6 +94,17 @@ def _run(what: str, fn, device, *args):
 
 # ---- selective scan --------------------------------------------------------------------------
 
+@functools.lru_cache(maxsize=256)
+def _scan_workspaces(device, b, t, d, n, g, io, chunk):
+    """Bytes of the kept states, and of a forward's and a backward's scratch: they go by the sizes (and the device) alone."""
+    sizes = [ctypes.c_size_t() for _ in range(3)]
+    record = _SCAN.pack(b, t, d, n, g, 0, io, chunk, *[0] * 41)
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().atlas_sscan_workspace(record, *[ctypes.byref(s) for s in sizes]),
+                   "selective_scan workspace")
+    return tuple(s.value for s in sizes)
+
+
 class _Scan:
     """The operands of one scan call, ready for the C ABI."""
 
@@ -116,10 +128,8 @@ class _Scan:
             _ptr(du), _ptr(ddelta), _ptr(dz), _ptr(dB), _ptr(dC), _ptr(dA), _ptr(dD), _ptr(dbias), _ptr(dh0))
 
     def workspaces(self):
-        s, f, b = ctypes.c_size_t(), ctypes.c_size_t(), ctypes.c_size_t()
-        _lib.check(_lib.lib().atlas_sscan_workspace(self.pack(), ctypes.byref(s), ctypes.byref(f), ctypes.byref(b)),
-                   "selective_scan workspace")
-        return s.value, f.value, b.value
+        u = self.u
+        return _scan_workspaces(u.device.index, *u.shape, self.B.shape[3], self.B.shape[2], _IO[u.dtype], self.chunk)
 
     def forward(self, keep: bool):
         """(out, final state, kept states or None)."""
