@@ -136,21 +136,20 @@ struct Feed {
       bytes = n;
     }
   }
-  __device__ __forceinline__ void tile(IO* dst, int64_t stride, int rows, int vec, int lane) const {
-    if (vec) {
+  __device__ __forceinline__ void vectors(IO* dst, int64_t stride, int rows, int lane) const {
 #pragma unroll
-      for (int i = 0; i < ROWS; i += STEP) {
-        const int r = lane / PER + i;
-        if (ROWS % STEP != 0 && r >= ROWS) break;
-        cp_piece<E * (int)sizeof(IO)>(dst + r * W + lane % PER * E, p + i * stride, r < rows ? bytes : 0);
-      }
-    } else {
+    for (int i = 0; i < ROWS; i += STEP) {
+      const int r = lane / PER + i;
+      if (ROWS % STEP != 0 && r >= ROWS) break;
+      cp_piece<E * (int)sizeof(IO)>(dst + r * W + lane % PER * E, p + i * stride, r < rows ? bytes : 0);
+    }
+  }
+  __device__ __forceinline__ void elements(IO* dst, int64_t stride, int rows, int lane) const {
 #pragma unroll 4
-      for (int at = lane; at < ROWS * W; at += 32) {
-        const int r = at / W, c = at % W;
-        if (r < rows && c < bytes) dst[at] = p[r * stride + c];
-        else from_f(dst[at], 0.f);
-      }
+    for (int at = lane; at < ROWS * W; at += 32) {
+      const int r = at / W, c = at % W;
+      if (r < rows && c < bytes) dst[at] = p[r * stride + c];
+      else from_f(dst[at], 0.f);
     }
   }
 };

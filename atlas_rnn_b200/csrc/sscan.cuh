@@ -20,6 +20,8 @@
 // that enter the chunks (each earlier one decayed by exp(A sum dt)), and the pass over the outputs starts from those.
 // That pays the exponentials twice.
 #pragma once
+#include <type_traits>
+
 #include "row_ops.cuh"
 
 namespace atlas {
@@ -258,19 +260,25 @@ __global__ void __launch_bounds__(32 * kWarps, kFwdCtas) k_sscan_fwd(const ScanA
   Cols fc((const IO*)a.Cm + w.b * a.C_sb + w.g * a.C_sg + t_lo * a.C_st, a.C_st, a.N, a.vecbc, lane);
   auto fetch = [&](int rows, int s) {  // the next tile
     auto& r = sm.raw[s];
-    fd.tile(&r.rows[0][0][0], a.d_st, rows, a.vec, lane);
-    fu.tile(&r.rows[1][0][0], a.u_st, rows, a.vec, lane);
-    fd.p += kTT * a.d_st, fu.p += kTT * a.u_st;
-    if (Z) {
-      fz.tile(&r.rows[SM::kRows - 1][0][0], a.z_st, rows, a.vec, lane);
-      fz.p += kTT * a.z_st;
+    if (a.vec) {
+      fd.vectors(&r.rows[0][0][0], a.d_st, rows, lane);
+      fu.vectors(&r.rows[1][0][0], a.u_st, rows, lane);
+      if (Z) fz.vectors(&r.rows[SM::kRows - 1][0][0], a.z_st, rows, lane);
+    } else {
+      fd.elements(&r.rows[0][0][0], a.d_st, rows, lane);
+      fu.elements(&r.rows[1][0][0], a.u_st, rows, lane);
+      if (Z) fz.elements(&r.rows[SM::kRows - 1][0][0], a.z_st, rows, lane);
     }
-    fb.tile(&r.bc[0][0][0], a.B_st, rows, a.vecbc, lane);
-    fb.p += kTT * a.B_st;
-    if (!ENDS) {
-      fc.tile(&r.bc[SM::kBC - 1][0][0], a.C_st, rows, a.vecbc, lane);
-      fc.p += kTT * a.C_st;
+    if (a.vecbc) {
+      fb.vectors(&r.bc[0][0][0], a.B_st, rows, lane);
+      if (!ENDS) fc.vectors(&r.bc[SM::kBC - 1][0][0], a.C_st, rows, lane);
+    } else {
+      fb.elements(&r.bc[0][0][0], a.B_st, rows, lane);
+      if (!ENDS) fc.elements(&r.bc[SM::kBC - 1][0][0], a.C_st, rows, lane);
     }
+    fd.p += kTT * a.d_st, fu.p += kTT * a.u_st, fb.p += kTT * a.B_st;
+    if (Z) fz.p += kTT * a.z_st;
+    if (!ENDS) fc.p += kTT * a.C_st;
     cp_commit();
   };
   int left = t_live > t_lo ? (int)(t_live - t_lo) : 0;  // steps to walk
@@ -336,16 +344,22 @@ __global__ void __launch_bounds__(32 * kWarps, kFwdCtas) k_sscan_fwd(const ScanA
     }
     __syncwarp();
     if (!ENDS) {
+      auto rows_out = [&](auto whole_tile_) {  // every row and channel pair of the tile, or those that there are
+        constexpr bool whole_tile = decltype(whole_tile_)::value;
 #pragma unroll
-      for (int k = 0; k < kTT; k += PR) {
-        const int tt = pr + k;
-        f2 y = fma2(skip, ld2(&raw.rows[1][tt][pc]), ld2(&sm.y[tt][pc]));
-        if (Z) {
-          const f2 z = ld2(&raw.rows[SM::kRows - 1][tt][pc]);
-          y = mul2(y, mul2(z, sigmoid_2(z)));
+        for (int k = 0; k < kTT; k += PR) {
+          const int tt = pr + k;
+          f2 y = fma2(skip, ld2(&raw.rows[1][tt][pc]), ld2(&sm.y[tt][pc]));
+          if (Z) {
+            const f2 z = ld2(&raw.rows[SM::kRows - 1][tt][pc]);
+            y = mul2(y, mul2(z, sigmoid_2(z)));
+          }
+          if (whole_tile) st2(out + k * (int64_t)a.Dm, y);
+          else if (tt < rows) store2(out + k * (int64_t)a.Dm, y, whole, c0, c1);
         }
-        if (tt < rows) store2(out + k * (int64_t)a.Dm, y, whole, c0, c1);
-      }
+      };
+      if (whole && rows >= kTT) rows_out(std::true_type());
+      else rows_out(std::false_type());
       out += kTT * (int64_t)a.Dm;
       __syncwarp();  // the fetch after next writes these rows
     }
@@ -534,15 +548,19 @@ __global__ void __launch_bounds__(32 * kWarps) k_sscan_bwd_ends(const ScanArgs a
   Feed<IO, kTT, NP> fc((const IO*)a.Cm + w.b * a.C_sb + w.g * a.C_sg + t_at * a.C_st, a.C_st, a.N, a.vecbc, lane);
   auto fetch = [&](int rows, int s) {
     auto& r = sm.raw[s];
-    fd.tile(&r.rows[0][0][0], a.d_st, rows, a.vec, lane);
-    fo.tile(&r.rows[1][0][0], a.o_st, rows, a.vec, lane);
-    fd.p -= kTT * a.d_st, fo.p -= kTT * a.o_st;
-    if (Z) {
-      fz.tile(&r.rows[Z ? 2 : 0][0][0], a.z_st, rows, a.vec, lane);
-      fz.p -= kTT * a.z_st;
+    if (a.vec) {
+      fd.vectors(&r.rows[0][0][0], a.d_st, rows, lane);
+      fo.vectors(&r.rows[1][0][0], a.o_st, rows, lane);
+      if (Z) fz.vectors(&r.rows[Z ? 2 : 0][0][0], a.z_st, rows, lane);
+    } else {
+      fd.elements(&r.rows[0][0][0], a.d_st, rows, lane);
+      fo.elements(&r.rows[1][0][0], a.o_st, rows, lane);
+      if (Z) fz.elements(&r.rows[Z ? 2 : 0][0][0], a.z_st, rows, lane);
     }
-    fc.tile(&r.bc[0][0], a.C_st, rows, a.vecbc, lane);
-    fc.p -= kTT * a.C_st;
+    if (a.vecbc) fc.vectors(&r.bc[0][0], a.C_st, rows, lane);
+    else fc.elements(&r.bc[0][0], a.C_st, rows, lane);
+    fd.p -= kTT * a.d_st, fo.p -= kTT * a.o_st, fc.p -= kTT * a.C_st;
+    if (Z) fz.p -= kTT * a.z_st;
     cp_commit();
   };
   if (ntile) fetch((int)(t_live - t_at), 0);
@@ -647,18 +665,27 @@ __global__ void __launch_bounds__(32 * kWarps, kBwdCtas) k_sscan_bwd(const ScanA
   Feed<float, CH, NP> fh(a.hsave + ((w.b * nblk + t_at / kTT) * a.Dm + w.d0) * NP, NP, NP, 1, lane);
   auto fetch = [&](int rows, int s) {
     auto& r = sm.raw[s];
-    fd.tile(&r.rows[0][0][0], a.d_st, rows, a.vec, lane);
-    fu.tile(&r.rows[1][0][0], a.u_st, rows, a.vec, lane);
-    fo.tile(&r.rows[2][0][0], a.o_st, rows, a.vec, lane);
-    fd.p -= kTT * a.d_st, fu.p -= kTT * a.u_st, fo.p -= kTT * a.o_st;
-    if (Z) {
-      fz.tile(&r.rows[Z ? 3 : 0][0][0], a.z_st, rows, a.vec, lane);
-      fz.p -= kTT * a.z_st;
+    if (a.vec) {
+      fd.vectors(&r.rows[0][0][0], a.d_st, rows, lane);
+      fu.vectors(&r.rows[1][0][0], a.u_st, rows, lane);
+      fo.vectors(&r.rows[2][0][0], a.o_st, rows, lane);
+      if (Z) fz.vectors(&r.rows[Z ? 3 : 0][0][0], a.z_st, rows, lane);
+    } else {
+      fd.elements(&r.rows[0][0][0], a.d_st, rows, lane);
+      fu.elements(&r.rows[1][0][0], a.u_st, rows, lane);
+      fo.elements(&r.rows[2][0][0], a.o_st, rows, lane);
+      if (Z) fz.elements(&r.rows[Z ? 3 : 0][0][0], a.z_st, rows, lane);
     }
-    fb.tile(&sm.bc[0][0][0], a.B_st, rows, a.vecbc, lane);
-    fc.tile(&sm.bc[1][0][0], a.C_st, rows, a.vecbc, lane);
-    fb.p -= kTT * a.B_st, fc.p -= kTT * a.C_st;
-    fh.tile(&r.h[0][0], NP, w.nc, 1, lane);
+    if (a.vecbc) {
+      fb.vectors(&sm.bc[0][0][0], a.B_st, rows, lane);
+      fc.vectors(&sm.bc[1][0][0], a.C_st, rows, lane);
+    } else {
+      fb.elements(&sm.bc[0][0][0], a.B_st, rows, lane);
+      fc.elements(&sm.bc[1][0][0], a.C_st, rows, lane);
+    }
+    fh.vectors(&r.h[0][0], NP, w.nc, lane);
+    fd.p -= kTT * a.d_st, fu.p -= kTT * a.u_st, fo.p -= kTT * a.o_st, fb.p -= kTT * a.B_st, fc.p -= kTT * a.C_st;
+    if (Z) fz.p -= kTT * a.z_st;
     fh.p -= (int64_t)a.Dm * NP;
     cp_commit();
   };
@@ -790,28 +817,40 @@ __global__ void __launch_bounds__(32 * kWarps, kBwdCtas) k_sscan_bwd(const ScanA
     __syncwarp();
 
     // the tile's rows: du, ddelta, dz; their share of d D and d bias
+    auto rows_out = [&](auto whole_tile_) {
+      constexpr bool whole_tile = decltype(whole_tile_)::value;
 #pragma unroll
-    for (int k = 0; k < kTT; k += PR) {
-      const int tt = pr + k;
-      const f2 u = ld2(&raw.rows[1][tt][pc]), dy = ld2(&sm.dy[tt][pc]), s1 = ld2(&sm.y[0][tt][pc]);
-      const f2 du = fma2(ld2(&sm.dt[tt][pc]), s1, mul2(skip, dy));
-      f2 dd = fma2(u, s1, mul2(ld2(&sm.y[1][tt][pc]), both(0.6931471805599453f)));
-      if (a.softplus) dd = mul2(dd, sigmoid_2(add2(ld2(&raw.rows[0][tt][pc]), bias)));
-      const int64_t o = at + k * (int64_t)a.Dm;
-      if (tt < rows) {
-        store2((IO*)a.du + o, du, whole, c0, c1);
-        store2((IO*)a.ddelta + o, dd, whole, c0, c1);
-        accD = fma2(dy, u, accD);
-        accb = add2(accb, dd);
+      for (int k = 0; k < kTT; k += PR) {
+        const int tt = pr + k;
+        const f2 u = ld2(&raw.rows[1][tt][pc]), dy = ld2(&sm.dy[tt][pc]), s1 = ld2(&sm.y[0][tt][pc]);
+        const f2 du = fma2(ld2(&sm.dt[tt][pc]), s1, mul2(skip, dy));
+        f2 dd = fma2(u, s1, mul2(ld2(&sm.y[1][tt][pc]), both(0.6931471805599453f)));
+        if (a.softplus) dd = mul2(dd, sigmoid_2(add2(ld2(&raw.rows[0][tt][pc]), bias)));
+        f2 dz = 0;
+        if (Z) {
+          const f2 z = ld2(&raw.rows[Z ? 3 : 0][tt][pc]), sg = sigmoid_2(z);
+          const f2 y = fma2(skip, u, ld2(&sm.y[Z ? 2 : 0][tt][pc]));
+          // silu'(z) = sg (1 + z (1 - sg))
+          dz = mul2(mul2(ld2(&raw.rows[2][tt][pc]), y), mul2(sg, fma2(z, fma2(sg, both(-1.f), both(1.f)), both(1.f))));
+        }
+        const int64_t o = at + k * (int64_t)a.Dm;
+        if (whole_tile || tt < rows) {
+          accD = fma2(dy, u, accD);
+          accb = add2(accb, dd);
+          if (whole_tile) {
+            st2((IO*)a.du + o, du);
+            st2((IO*)a.ddelta + o, dd);
+            if (Z) st2((IO*)a.dz + o, dz);
+          } else {
+            store2((IO*)a.du + o, du, whole, c0, c1);
+            store2((IO*)a.ddelta + o, dd, whole, c0, c1);
+            if (Z) store2((IO*)a.dz + o, dz, whole, c0, c1);
+          }
+        }
       }
-      if (Z) {
-        const f2 z = ld2(&raw.rows[Z ? 3 : 0][tt][pc]), sg = sigmoid_2(z);
-        const f2 y = fma2(skip, u, ld2(&sm.y[Z ? 2 : 0][tt][pc]));
-        // silu'(z) = sg (1 + z (1 - sg))
-        const f2 sl = mul2(sg, fma2(z, fma2(sg, both(-1.f), both(1.f)), both(1.f)));
-        if (tt < rows) store2((IO*)a.dz + o, mul2(mul2(ld2(&raw.rows[2][tt][pc]), y), sl), whole, c0, c1);
-      }
-    }
+    };
+    if (whole && rows >= kTT) rows_out(std::true_type());
+    else rows_out(std::false_type());
     at -= kTT * (int64_t)a.Dm;
     __syncthreads();  // one a tile: the records of the other buffer are written next
 #pragma unroll
