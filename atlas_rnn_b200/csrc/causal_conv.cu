@@ -21,7 +21,7 @@ int ygrid_of(int64_t T, int run) { return (int)((T + (int64_t)run * kConvWarps -
 
 bool shape_ok(int K, int dtype, int64_t B, int64_t T, int64_t C) {
   return K >= 2 && K <= 8 && (dtype == ATLAS_F32 || dtype == ATLAS_BF16) && B >= 1 && T >= 1 && C >= 1 &&
-         C <= ((int64_t)1 << 20) && T <= ((int64_t)1 << 31) &&
+         C <= ((int64_t)1 << 20) && T <= 0x7fffffff &&
          B <= 0x7fffffff / std::max(1, ygrid_of(T, 8));
 }
 bool wide(const void* p, int64_t sb, int64_t st, int size, int W) {

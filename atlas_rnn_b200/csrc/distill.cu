@@ -15,7 +15,7 @@ namespace {
 
 bool pack(const AtlasDistill* p, DistillArgs& a, int& C) {
   if (!p || !p->logits || !p->values || !p->indices || !p->stats || p->rows < 1 || p->V < 1 || p->V > 0x7ffffff0 ||
-      p->K < 1 || p->K > kMaxK || (p->dtype != ATLAS_F32 && p->dtype != ATLAS_BF16) || !(p->temperature > 0.f) ||
+      p->K < 1 || p->K > kMaxK || (p->dtype != ATLAS_F32 && p->dtype != ATLAS_BF16) || !(p->temperature >= 0.99e-6f && p->temperature <= 1.01e6f) ||
       p->rows > 0x7fffffff / 8 || (uintptr_t)p->stats % 16)
     return false;
   a.logits = p->logits, a.stride = p->stride, a.values = p->values, a.indices = p->indices;
@@ -37,7 +37,7 @@ int fwd(const DistillArgs& a, int64_t rows, int C, cudaStream_t st) {
   cfg.gridDim = dim3((unsigned)(rows * C));
   cfg.blockDim = dim3(NT);
   cfg.stream = st;
-  cfg.attrs = &at, cfg.numAttrs = 1;
+  cfg.attrs = &at, cfg.numAttrs = C > 1;
   const int slot = prof_begin(KID_DISTILL_FWD, st);
   if (cudaLaunchKernelEx(&cfg, k_distill_fwd<IO, NT>, a) != cudaSuccess) return ATLAS_ERR_LAUNCH;
   LAUNCH_CHECK();

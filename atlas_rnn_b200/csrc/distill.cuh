@@ -17,6 +17,7 @@ namespace dst {
 
 namespace cg = cooperative_groups;
 constexpr int kMaxK = 1024;
+constexpr int kMarks = 512;  // words of a bitmap of tokens, by their low bits
 
 struct DistillArgs {
   const void* logits;
@@ -180,12 +181,16 @@ __global__ void __launch_bounds__(NT) k_distill_fwd(const DistillArgs a) {
   }
 }
 
-// grid (splits, rows): every CTA its own part of a row
+// grid rows x splits: every CTA its own part of a row. The sums over equal tokens: two bitmaps of
+// the entries' low bits (seen, seen again) clear most of being repeated, and a warp looks together through all entries for
+// each of the others (8192 x 32000, bf16: 172 us with 20 entries, 217 with 256, 399 with 1024; with every entry looking
+// through all of them 172, 238 and 1500).
 template <class IO, int NT>
 __global__ void __launch_bounds__(NT) k_distill_bwd(const DistillArgs a, int C) {
   constexpr int E = 16 / (int)sizeof(IO), U = 4;
   __shared__ float s_p[kMaxK];
   __shared__ int s_t[kMaxK];
+  __shared__ unsigned s_seen[kMarks], s_again[kMarks];
   const int64_t row = blockIdx.x / C;
   const int rank = (int)(blockIdx.x - row * C), tid = threadIdx.x;
   const int lo = rank * a.split, n = a.V - lo < a.split ? (a.V - lo < 0 ? 0 : a.V - lo) : a.split;
@@ -194,9 +199,15 @@ __global__ void __launch_bounds__(NT) k_distill_bwd(const DistillArgs a, int C) 
   const bool some = st.w > 0.f;
   const IO* x = (const IO*)a.logits + row * a.stride;
   IO* o = (IO*)a.dlogits + row * a.V;
+  for (int i = tid; i < kMarks; i += NT) s_seen[i] = s_again[i] = 0;
+  __syncthreads();
   for (int k = tid; k < a.K; k += NT) {
     int64_t t;
     const float v = entry(a, row, k, t);
+    if (v > -INFINITY) {
+      const unsigned w = (unsigned)t / 32 % kMarks, bit = 1u << (t & 31);
+      if (atomicOr(&s_seen[w], bit) & bit) atomicOr(&s_again[w], bit);
+    }
     s_t[k] = v > -INFINITY ? (int)t : -1;
     s_p[k] = v > -INFINITY ? weight(v, st.z, c) / st.w : 0.f;
   }
@@ -228,11 +239,20 @@ __global__ void __launch_bounds__(NT) k_distill_bwd(const DistillArgs a, int C) 
     ss::from_f(ol[at], grad(ss::to_f(xl[at])));
   }
   __syncthreads();  // the entries' own values go over those above; equal tokens write the same sum
-  for (int k = tid; k < a.K; k += NT) {
-    const int t = s_t[k];
-    if (t < lo || t >= lo + n) continue;
-    float p = 0.f;
-    for (int j = 0; j < a.K; ++j) p += s_t[j] == t ? s_p[j] : 0.f;
+  const int lane = tid & 31;
+  for (int k = tid; k - lane < a.K; k += NT) {
+    const int t = k < a.K ? s_t[k] : -1;
+    const bool mine = t >= lo && t < lo + n;
+    float p = mine ? s_p[k] : 0.f;
+    unsigned again = __ballot_sync(0xffffffffu, mine && s_again[(unsigned)t / 32 % kMarks] >> (t & 31) & 1);
+    for (; again; again &= again - 1) {
+      const int l = __ffs(again) - 1, tl = __shfl_sync(0xffffffffu, t, l);
+      float q = 0.f;
+      for (int j = lane; j < a.K; j += 32) q += s_t[j] == tl ? s_p[j] : 0.f;
+      q = warp_reduce(q, add_op);
+      if (lane == l) p = q;
+    }
+    if (!mine) continue;
     ss::from_f(o[t], g * (ss::ex2(fmaf(ss::to_f(x[t]) - st.x, c, -st.y)) - p));
   }
 }

@@ -63,7 +63,7 @@ int launch(SampleArgs a, int64_t rows, cudaStream_t st) {
 }  // namespace
 
 extern "C" int atlas_sample_tokens(const AtlasSample* p, void* stream) {
-  if (!p || !p->logits || !p->noise || !p->out || p->rows < 1 || p->V < 1 || p->V > 0x7ffffff0 ||
+  if (!p || !p->logits || !p->noise || !p->out || p->rows < 1 || p->V < 1 || p->V > kMaxV ||
       (p->dtype != ATLAS_F32 && p->dtype != ATLAS_BF16) || p->rows > 0x7fffffff / 8)
     return ATLAS_ERR_INVALID_ARG;
   SampleArgs a = {};

@@ -35,6 +35,7 @@ using u64 = unsigned long long;
 constexpr int kBins = 2048, kCap = 2048;
 constexpr int kFastK = 512;
 constexpr int kNone = 0x7fffffff;
+constexpr int kMaxV = (1 << 24) - 16;  // as many masses of up to 2^40 add up to less than 2^64
 
 struct SampleArgs {
   const void* logits;  // [rows, V], rows `stride` elements apart
@@ -240,9 +241,9 @@ __global__ void __launch_bounds__(NT) k_sample(const SampleArgs a) {
   const double top_p = a.top_p_row ? (double)a.top_p_row[row] : a.top_p;
   const double min_p = a.min_p_row ? (double)a.min_p_row[row] : a.min_p;
   int64_t k = a.top_k_row ? a.top_k_row[row] : a.top_k;
-  if (!(top_p > 0.0) || !(min_p <= 1.0) || !(temperature > 0.0)) k = 1;  // nothing but the first token
+  if (!(top_p > 0.0) || !(min_p <= 1.0) || !(temperature >= 1e-30)) k = 1;  // nothing but the first token
   const bool need_k = k >= 1 && k < a.V, need_p = top_p < 1.0;
-  const float inv_t = (float)fmin(1.0 / temperature, 1e30);  // beyond: settled in fp64 by Best
+  const float inv_t = (float)(1.0 / fmax(temperature, 1e-30));
 
   auto block_max = [&](float v) {
     const float wm = warp_reduce(v, fmax_op);

@@ -57,10 +57,12 @@ Plan bwd_plan(const AtlasSelScan* a) {
 bool sizes_ok(const AtlasSelScan* a) {
   return a && a->B >= 1 && a->T >= 1 && a->D >= 1 && a->N >= 1 && a->N <= 64 && a->G >= 1 && a->D % a->G == 0 &&
          (a->dtype_io == ATLAS_F32 || a->dtype_io == ATLAS_BF16) && a->chunk >= 0 && a->chunk % 32 == 0 &&
-         a->B <= (1 << 24) && a->T <= ((int64_t)1 << 40) &&
+         a->B <= (1 << 24) && a->T <= 0x7fffffff && a->D <= (1 << 30) &&
          a->B * (int64_t)a->D * (a->N / 4 + 8) < ((int64_t)1 << 36);
 }
-bool inputs_ok(const AtlasSelScan* a) { return a->u && a->delta && a->Bm && a->Cm && a->A; }
+bool inputs_ok(const AtlasSelScan* a) {
+  return a->u && a->delta && a->Bm && a->Cm && a->A && (uintptr_t)a->saved % 16 == 0 && (uintptr_t)a->scratch % 16 == 0;
+}
 
 size_t saved_bytes(const AtlasSelScan* a) {
   return (size_t)a->B * ((a->T + kTT - 1) / kTT) * a->D * padded(a->N) * sizeof(float);

@@ -20,6 +20,7 @@
 // that enter the chunks (each earlier one decayed by exp(A sum dt)), and the pass over the outputs starts from those.
 // That pays the exponentials twice.
 #pragma once
+#include <cfloat>
 #include <type_traits>
 
 #include "row_ops.cuh"
@@ -112,11 +113,17 @@ struct Block {
   }
 };
 
+// A in units of log2. -inf is the lowest finite value: dt A is 0, not NaN, at the steps that a tile or a chunk has too
+// many, whose dt is 0.
+__device__ __forceinline__ float log2_decay(float A) {
+  const float v = A * kLog2e;
+  return v < -FLT_MAX ? -FLT_MAX : v;
+}
 // A [Dm, N] in units of log2.
 template <int MC, int CH>
 __device__ __forceinline__ void load_A(const ScanArgs& a, const Place<CH>& w, int c4, int n4, Block<MC>& A) {
   A.fill([&](int c, int i) {
-    return c4 + c < w.nc && n4 + i < a.N ? a.A[(w.d0 + c4 + c) * a.N + n4 + i] * kLog2e : 0.f;
+    return c4 + c < w.nc && n4 + i < a.N ? log2_decay(a.A[(w.d0 + c4 + c) * a.N + n4 + i]) : 0.f;
   });
 }
 // A state [B, Dm, N] (null: zeros).
@@ -391,7 +398,7 @@ __global__ void __launch_bounds__(kCarryThr) k_sscan_carry(const ScanArgs a) {
   float A[4], h[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    A[k] = n4 + k < a.N ? a.A[(int64_t)d * a.N + n4 + k] * kLog2e : 0.f;
+    A[k] = n4 + k < a.N ? log2_decay(a.A[(int64_t)d * a.N + n4 + k]) : 0.f;
     h[k] = s && n4 + k < a.N ? s[row * a.N + n4 + k] : 0.f;
   }
   // the record that enters last has no end state: chunk nchunk - 1 (BACK: 0)
@@ -463,15 +470,15 @@ __global__ void __launch_bounds__(kStepThr) k_sscan_step(const ScanArgs a) {
     const int64_t b = (int64_t)blockIdx.y * R + r;
     const bool live = len[r] > 0;
     float hv[4] = {h[r].x, h[r].y, h[r].z, h[r].w}, y = 0.f;
-    const float Av[4] = {A.x, A.y, A.z, A.w}, u = live ? to_f(du[r]) : 0.f;
+    const float Av[4] = {log2_decay(A.x), log2_decay(A.y), log2_decay(A.z), log2_decay(A.w)}, u = live ? to_f(du[r]) : 0.f;
     float x = to_f(dd_[r]) + bias;
     if (a.softplus) x = softplus(x);
     if (!live) x = 0.f;
-    const float xl = x * kLog2e, xu = x * u;
+    const float xu = x * u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float Bv = live ? to_f(B[r].v[i]) : 0.f, Cv = live ? to_f(C[r].v[i]) : 0.f;
-      hv[i] = fmaf(ex2(Av[i] * xl), hv[i], xu * Bv);
+      hv[i] = fmaf(ex2(Av[i] * x), hv[i], xu * Bv);
       if (V4 ? on : n4 + i < a.N) y = fmaf(Cv, hv[i], y);
     }
 #pragma unroll

@@ -60,7 +60,8 @@ def distill_loss(logits: Tensor, teacher_values: Tensor, teacher_indices: Tensor
     logits [..., V] (float32 or bfloat16); teacher_values [..., K] (a floating type) and teacher_indices [..., K] (int32 or
     int64), K up to 1024: the teacher's logits and their tokens. Entries whose index is outside 0 .. V - 1 (-1, say), or
     whose value is -inf or NaN, are absent, so rows may have fewer than K; tokens may repeat. Per row, with
-    p = softmax(teacher_values / temperature) over the entries and q = softmax(logits / temperature):
+    p = softmax(teacher_values / temperature) over the entries and q = softmax(logits / temperature), temperature from
+    1e-6 to 1e6:
 
         loss = temperature^2 sum_k p_k (log p_k - log q[index_k])
 
@@ -80,8 +81,8 @@ def distill_loss(logits: Tensor, teacher_values: Tensor, teacher_indices: Tensor
         raise TypeError(f"atlas_rnn_b200.{what}: teacher_indices must be int32 or int64, not {teacher_indices.dtype}")
     if reduction not in ("none", "mean", "sum"):
         raise ValueError(f"atlas_rnn_b200.{what}: reduction must be 'none', 'mean' or 'sum', not {reduction!r}")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"atlas_rnn_b200.{what}: temperature must be positive and finite, not {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"atlas_rnn_b200.{what}: temperature must be from 1e-6 to 1e6, not {temperature}")
     lead, V, K = logits.shape[:-1], logits.shape[-1], teacher_values.shape[-1]
     if V > 0x7ffffff0:
         raise ValueError(f"atlas_rnn_b200.{what}: {V} tokens are too many")

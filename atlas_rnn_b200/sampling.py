@@ -5,6 +5,7 @@
 """
 from __future__ import annotations
 
+import operator
 import struct
 
 import torch
@@ -13,6 +14,8 @@ from torch import Tensor
 from . import _lib
 from .selective_scan import _IO, _check, _need_cuda, _ptr, _run
 
+MAX_VOCAB = (1 << 24) - 16  # tokens per row
+
 # struct AtlasSample of include/atlas_mem.h in native alignment (checked against the header by the tests)
 _SAMPLE = struct.Struct("@3P4q3dq4Pi4x")
 
@@ -20,6 +23,8 @@ _SAMPLE = struct.Struct("@3P4q3dq4Pi4x")
 def _setting(name: str, value, lead: tuple, device, dtype, lowest, highest):
     """(one value, None) or (0, a tensor with one per row)."""
     if not isinstance(value, Tensor):
+        if dtype == torch.int32:
+            value = operator.index(value)  # TypeError for what is no integer
         if not (value >= lowest and (highest is None or value <= highest)):  # a NaN fails too
             raise ValueError(f"atlas_rnn_b200.sample_tokens: {name} must be at least {lowest}"
                              + (f" and at most {highest}" if highest is not None else "") + f", not {value}")
@@ -41,19 +46,20 @@ def sample_tokens(logits: Tensor, noise: Tensor, *, temperature=1.0, top_k=0, to
         top_p   of those, the ones with less than top_p of their probability before them, the first always (1: all)
         min_p   of those, the ones with at least min_p times the first one's probability
 
-    and the token is the kept one with the largest logits / temperature - log(-log(noise)); temperature 0 gives the first
-    token. The filters see the logits without the temperature, as ``min_p_filter`` before ``gumbel_sample`` does: divide
+    and the token is the kept one with the largest logits / temperature - log(-log(noise)); temperature 0 (or below
+    1e-30) gives the first token. The filters see the logits without the temperature, as ``min_p_filter`` before ``gumbel_sample`` does: divide
     the logits beforehand for filters on the tempered distribution. Each setting is a number or a tensor with one value
     per row. Masked tokens are -inf (NaN counts as -inf); a row with nothing above -inf gives 0.
-    Returns int64 [...]: the token of exact arithmetic on these inputs, whatever the batch."""
+    V up to 2^24 - 16. Returns int64 [...], the same whatever the batch: scores are compared in float64, the probabilities
+    that the filters add up are exact to 2^-23 each."""
     what = "sample_tokens"
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"atlas_rnn_b200.{what}: expected logits [..., V], got {tuple(logits.shape)}")
     if logits.dtype not in _IO:
         raise TypeError(f"atlas_rnn_b200.{what}: logits must be float32 or bfloat16, not {logits.dtype}")
     dev, lead, V = logits.device, logits.shape[:-1], logits.shape[-1]
-    if V > 0x7ffffff0:
-        raise ValueError(f"atlas_rnn_b200.{what}: {V} tokens are too many")
+    if V > MAX_VOCAB:
+        raise ValueError(f"atlas_rnn_b200.{what}: at most {MAX_VOCAB} tokens, not {V}")
     _check(what, "noise", noise, logits.shape, torch.float32, dev)
     t, t_row = _setting("temperature", temperature, lead, dev, torch.float32, 0.0, None)
     k, k_row = _setting("top_k", top_k, lead, dev, torch.int32, 0, None)
@@ -68,5 +74,5 @@ def sample_tokens(logits: Tensor, noise: Tensor, *, temperature=1.0, top_k=0, to
     u = u if u.stride(1) == 1 or V == 1 else u.contiguous()
     _run(what, _lib.lib().atlas_sample_tokens, dev,
          _SAMPLE.pack(x.data_ptr(), u.data_ptr(), out.data_ptr(), x.shape[0], V, x.stride(0), u.stride(0), t, p, m,
-                      min(int(k), 0x7fffffff), _ptr(t_row), _ptr(p_row), _ptr(m_row), _ptr(k_row), _IO[x.dtype]))
+                      min(k, 0x7fffffff), _ptr(t_row), _ptr(p_row), _ptr(m_row), _ptr(k_row), _IO[x.dtype]))
     return out

@@ -22,6 +22,7 @@ from . import _lib
 
 MAX_STATE = 64     # states per channel
 MAX_CONV_K = 8     # taps
+MAX_BATCH, MAX_STEPS, MAX_CHANNELS, MAX_CONV_CHANNELS = 1 << 24, (1 << 31) - 1, 1 << 30, 1 << 20
 
 _IO = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
@@ -47,6 +48,12 @@ def _check(what: str, name: str, t: Tensor, shape: tuple, dtype, device):
         raise RuntimeError(f"atlas_rnn_b200.{what}: {name} is on {t.device}, expected {device}")
 
 
+def _check_sizes(what: str, b: int, t: int, channels: int, most: int):
+    if b > MAX_BATCH or t > MAX_STEPS or channels > most:
+        raise ValueError(f"atlas_rnn_b200.{what}: at most {MAX_BATCH} rows of {MAX_STEPS} steps of {most} channels, not "
+                         f"{(b, t, channels)}")
+
+
 def _f32(what: str, name: str, t: Tensor | None, shape: tuple, device) -> Tensor | None:
     """A parameter or state as dense fp32."""
     if t is None:
@@ -70,7 +77,7 @@ def _lengths(what: str, lengths, batch: int, device) -> Tensor | None:
     if not isinstance(lengths, Tensor) or lengths.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"atlas_rnn_b200.{what}: lengths must be an int32 or int64 tensor")
     _check(what, "lengths", lengths, (batch,), None, device)
-    return lengths.clamp(max=0x7fffffff).to(torch.int32).contiguous() if lengths.dtype == torch.int64 \
+    return lengths.clamp(0, 0x7fffffff).to(torch.int32).contiguous() if lengths.dtype == torch.int64 \
         else lengths.contiguous()
 
 
@@ -197,7 +204,8 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D:
 
     u, delta, z [b, t, d] and B, C [b, t, n] or [b, t, g, n] (d a multiple of g, n up to 64) are all float32 or all
     bfloat16, of any batch and step strides (halves of one projection are taken as they are); A [d, n],
-    D, delta_bias [d] and initial_state [b, d, n] are computed in float32, as is the state. lengths [b] (int32 or
+    D, delta_bias [d] and initial_state [b, d, n] are computed in float32, as is the state (an A of -inf as the lowest finite
+    value, so that a step with dt = 0 leaves the state). lengths [b] (int32 or
     int64): steps at or past a row's length are not read, leave its state alone and give 0.
     Returns (out [b, t, d] in u's type, final state [b, d, n] float32); both carry gradients to every
     floating input. The sums over steps, states and channels are in float32 and in a fixed order, so the same call gives the
@@ -215,6 +223,7 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D:
     b, t, d = u.shape
     g, n = B.shape[2], B.shape[3]
     dev = u.device
+    _check_sizes(what, b, t, d, MAX_CHANNELS)
     if not 1 <= n <= MAX_STATE:
         raise ValueError(f"atlas_rnn_b200.{what}: 1 to {MAX_STATE} states per channel, not {n}")
     if g < 1 or d % g:
@@ -304,6 +313,7 @@ def causal_conv1d(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, acti
     if activation not in (None, "silu"):
         raise ValueError(f"atlas_rnn_b200.{what}: activation must be None or 'silu', not {activation!r}")
     B, T, C = x.shape
+    _check_sizes(what, B, T, C, MAX_CONV_CHANNELS)
     K = weight.shape[-1]
     if not 2 <= K <= MAX_CONV_K:
         raise ValueError(f"atlas_rnn_b200.{what}: 2 to {MAX_CONV_K} taps, not {K}")

@@ -416,7 +416,8 @@ int atlas_omega_store_backward(const float* beta, const void* surprise, const fl
  * Bm / Cm, group (_sg); channels and states are dense. All other arrays are dense: A [D,N], Dskip, bias [D],
  * h0, hT and their gradients [B,D,N] in fp32; out, du, ddelta, dz [B,T,D] and dB, dC [B,T,G,N] in dtype_io.
  * len [B] (int32, NULL: T): steps at or past a row's length leave the state alone, give out = 0 and
- * zero gradients, and are not read. 1 <= N <= 64, D a multiple of G. */
+ * zero gradients, and are not read. 1 <= N <= 64, D a multiple of G, T < 2^31, D <= 2^30, B <= 2^24. An A of -inf is taken
+ * as the lowest finite value. `saved` and `scratch` are 16-byte aligned. */
 typedef struct AtlasSelScan {
   int64_t B, T;
   int32_t D, N, G;
@@ -449,7 +450,8 @@ int atlas_sscan_backward(const AtlasSelScan* a, void* stream);
  *   y[b,t,c] = act(bias[c] + sum_{j<K} w[c,j] x[b, t + j - (K-1), c]),
  * x at steps -(K-1) .. -1 from init [B,K-1,C] (NULL: zeros); silu 0: no activation. final [B,K-1,C] holds
  * the last K-1 inputs up to the row's length. x has element strides x_sb, x_st (channels dense); w [C,K],
- * bias [C] (NULL: 0) are fp32; the other arrays are dense, in dtype_io. len as above (y = 0 past it). 2 <= K <= 8. */
+ * bias [C] (NULL: 0) are fp32; the other arrays are dense, in dtype_io. len as above (y = 0 past it). 2 <= K <= 8,
+ * T < 2^31, C <= 2^20. */
 int atlas_causal_conv_forward(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias,
                               const void* init, const int32_t* len, void* y, void* final_state, int K, int silu,
                               int dtype_io, int64_t B, int64_t T, int64_t C, void* stream);
@@ -470,7 +472,8 @@ int atlas_causal_conv_backward(const void* x, int64_t x_sb, int64_t x_st, const 
  *   top-p: of those, the tokens with less than top_p of their mass exp(logit) before them (the first always; >= 1: all);
  *   min-p: of those, the tokens with at least min_p times the first one's probability (the first always);
  *   out = argmax over the kept of logit / temperature - log(-log u), u from noise [rows, V] fp32 in [0, 1], clamped as
- *   gumbel_noise clamps (1e-20); temperature <= 0: the first token. A row without any logit above -inf gives 0.
+ *   gumbel_noise clamps (1e-20); a temperature below 1e-30: the first token. A row without any logit above -inf gives 0.
+ * V <= 2^24 - 16.
  * Each setting is one value, or an array of one per row where its _row pointer is given. */
 typedef struct AtlasSample {
   const void* logits;
@@ -490,7 +493,8 @@ int atlas_sample_tokens(const AtlasSample* a, void* stream);
  * indices int64 [rows, K]; absent where the index is outside 0 .. V-1 or the value is -inf or NaN):
  *   p = softmax(values / temperature) over the entries, q = softmax(x / temperature),
  *   loss = temperature^2 sum_k p_k (log p_k - log q[index_k]), 0 for a row without entries (valid = 0, else 1);
- *   dlogits [rows, V] = dloss temperature (q - sum of p at the token). Tokens may repeat. 1 <= K <= 1024.
+ *   dlogits [rows, V] = dloss temperature (q - sum of p at the token). Tokens may repeat. 1 <= K <= 1024, temperature
+ *   from 1e-6 to 1e6.
  * stats [rows, 4] fp32 (16-byte aligned) is written by the forward and read by the backward. */
 typedef struct AtlasDistill {
   const void* logits;

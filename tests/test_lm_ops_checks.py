@@ -204,3 +204,35 @@ def test_native_distill_refuses_bad_arguments(native_lib):
         raw = _DISTILL.pack(*[16] * 8, f["rows"], f["V"], f["K"], 5, f["t"], f["dt"])
         assert native_lib.atlas_distill_forward(raw, None) == 1 and native_lib.atlas_distill_backward(raw, None) == 1, bad
     assert native_lib.atlas_distill_forward(_DISTILL.pack(*[0] * 8, 1, 5, 2, 5, 1.0, 0), None) == 1
+
+
+def vast(*shape, dtype=torch.float32):
+    return torch.zeros((), dtype=dtype).expand(*shape)
+
+
+def test_sizes_beyond_the_kernels_are_refused():
+    for b, t, d in ((1, 1 << 31, 1), (1 << 24 | 1, 1, 1), (1, 1, 1 << 30 | 1)):
+        r = lambda *s: vast(b, t, *s)
+        with pytest.raises(ValueError, match="at most"):
+            A.selective_scan(r(d), r(d), vast(d, 4), r(4), r(4))
+    for b, t, c in ((1, 1 << 31, 1), (1 << 24 | 1, 1, 1), (1, 1, 1 << 20 | 1)):
+        with pytest.raises(ValueError, match="at most"):
+            A.causal_conv1d(vast(b, t, c), vast(c, 4))
+    with pytest.raises(ValueError, match="at most"):
+        A.sample_tokens(vast(1, 1 << 24), vast(1, 1 << 24))
+    with pytest.raises(TypeError):
+        A.sample_tokens(vast(1, 8), vast(1, 8), top_k=0.5)
+    for tau in (1e-7, 1e7, float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            A.distill_loss(vast(1, 8), vast(1, 2), vast(1, 2, dtype=torch.int64), temperature=tau)
+
+
+def test_native_calls_refuse_unaligned_workspaces(native_lib):
+    from atlas_rnn_b200.selective_scan import _SCAN
+    f = [1, 8, 4, 16, 1, 1, 0, 0] + [16] * 5 + [0] * 12 + [16, 0, 0, 0] + [0] + [16, 16] + [0] * 17
+    assert len(f) == 8 + 41
+    saved, scratch = 32, 33  # fields
+    for at in (saved, scratch):
+        g = list(f)
+        g[at] = 24
+        assert native_lib.atlas_sscan_forward(_SCAN.pack(*g), None) == 1
