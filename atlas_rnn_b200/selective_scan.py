@@ -254,7 +254,7 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D:
 
 def _conv_forward(x, w, bias, init, lengths, silu):
     B, T, C = x.shape
-    K = w.shape[1]
+    K = w.shape[-1]
     y = torch.empty(B, T, C, dtype=x.dtype, device=x.device)
     final = torch.empty(B, K - 1, C, dtype=x.dtype, device=x.device)
     _run("causal_conv1d forward", _lib.lib().atlas_causal_conv_forward, x.device, x.data_ptr(), x.stride(0),
@@ -277,13 +277,13 @@ class CausalConv1dFn(torch.autograd.Function):
     def backward(ctx, dy, d_final):
         x, w, bias, init, lengths = ctx.saved_tensors
         B, T, C = x.shape
-        K = w.shape[1]
+        K = w.shape[-1]
         dev = x.device
         dy = torch.zeros(B, T, C, dtype=x.dtype, device=dev) if dy is None else _rows(dy)
         d_final = None if d_final is None else d_final.contiguous()
         dx = torch.empty(B, T, C, dtype=x.dtype, device=dev)
         d_init = torch.empty_like(init) if init is not None and ctx.needs_input_grad[3] else None
-        dw = torch.empty(C, K, dtype=torch.float32, device=dev)
+        dw = torch.empty(w.shape, dtype=torch.float32, device=dev)
         dbias = torch.empty(C, dtype=torch.float32, device=dev) if bias is not None else None
         L = _lib.lib()
         scratch = torch.empty(L.atlas_causal_conv_scratch(B, T, C, K), dtype=torch.uint8, device=dev)
@@ -318,10 +318,8 @@ def causal_conv1d(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, acti
     if not 2 <= K <= MAX_CONV_K:
         raise ValueError(f"atlas_rnn_b200.{what}: 2 to {MAX_CONV_K} taps, not {K}")
     dev = x.device
-    if weight.dim() == 3:
-        _check(what, "weight", weight, (C, 1, K), None, dev)
-        weight = weight[:, 0]
-    w, bias = _f32(what, "weight", weight, (C, K), dev), _f32(what, "bias", bias, (C,), dev)
+    w = _f32(what, "weight", weight, (C, 1, K) if weight.dim() == 3 else (C, K), dev)
+    bias = _f32(what, "bias", bias, (C,), dev)
     if initial_state is not None:
         _check(what, "initial_state", initial_state, (B, K - 1, C), x.dtype, dev)
         if not initial_state.is_contiguous():
