@@ -429,15 +429,18 @@ __global__ void __launch_bounds__(kCarryThr) k_sscan_carry(const ScanArgs a) {
 // ---- one token ------------------------------------------------------------
 // T = 1 without a backward: a thread takes 4 neighbouring states (one 16-byte read and write of the state, which is the
 // traffic) of R batch rows, whose loads are all in flight together; LPC = NP / 4 lanes a channel. A, D and bias are read
-// once for the R rows. grid (channel blocks, row blocks).
+// once for the R rows. What a row needs once a channel (dt, the gate, the output) is done by one of the channel's lanes, R
+// rows by as many lanes. grid (channel blocks, row blocks).
 constexpr int kStepThr = 128;
 // V4: 16-byte accesses to A and the states, 4-element ones to B and C (N a multiple of 4)
 template <class IO, int NP, int R, bool V4>
 __global__ void __launch_bounds__(kStepThr) k_sscan_step(const ScanArgs a) {
-  constexpr int LPC = NP / 4;
-  const int d = blockIdx.x * (kStepThr / LPC) + threadIdx.x / LPC, n4 = threadIdx.x % LPC * 4;
+  constexpr int LPC = NP / 4, L = LPC < R ? LPC : R, RPL = R / L;  // lanes that take a row's own part; rows of each
+  const int l = threadIdx.x % LPC, d = blockIdx.x * (kStepThr / LPC) + threadIdx.x / LPC, n4 = l * 4;
   const bool on = d < a.Dm && (!V4 || n4 < a.N);
-  const int dd = d < a.Dm ? d : 0, nn = V4 && n4 < a.N ? n4 : 0, g = dd / (a.Dm / a.G);
+  const int dd = d < a.Dm ? d : 0, nn = V4 && n4 < a.N ? n4 : 0, g = a.G == 1 ? 0 : dd / (a.Dm / a.G);
+  const int64_t b0 = (int64_t)blockIdx.y * R;
+  const int left = a.Bsz - b0 < R ? (int)(a.Bsz - b0) : R, k0 = l % L * RPL;  // rows there are; the lane's first one
   auto four = [&](const float* p) {  // states n4 .. n4 + 3 of a row
     if (V4) return *reinterpret_cast<const float4*>(p + nn);
     return make_float4(n4 < a.N ? p[n4] : 0.f, n4 + 1 < a.N ? p[n4 + 1] : 0.f, n4 + 2 < a.N ? p[n4 + 2] : 0.f,
@@ -450,56 +453,76 @@ __global__ void __launch_bounds__(kStepThr) k_sscan_step(const ScanArgs a) {
   // all loads first, of rows that exist (what a dead row holds is dropped below), nothing used before the last is issued
   const float4 A = four(a.A + (int64_t)dd * a.N);
   const float bias = a.bias ? a.bias[dd] : 0.f, skip = a.D ? a.D[dd] : 0.f;
+  const float* h0 = a.h0 ? a.h0 + (b0 * a.Dm + dd) * a.N : nullptr;
+  const IO *pB = (const IO*)a.Bm + b0 * a.B_sb + g * a.B_sg, *pC = (const IO*)a.Cm + b0 * a.C_sb + g * a.C_sg;
   float4 h[R];
-  IO du[R], dd_[R], dz[R];
   Vec<IO, 4> B[R], C[R];
-  int len[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int64_t b = (int64_t)blockIdx.y * R + r < a.Bsz ? (int64_t)blockIdx.y * R + r : 0;
-    h[r] = a.h0 ? four(a.h0 + (b * a.Dm + dd) * a.N) : make_float4(0.f, 0.f, 0.f, 0.f);
-    du[r] = ((const IO*)a.u)[b * a.u_sb + dd];
-    dd_[r] = ((const IO*)a.delta)[b * a.d_sb + dd];
-    dz[r] = ((const IO*)(a.z ? a.z : a.u))[a.z ? b * a.z_sb + dd : 0];
-    B[r] = cols((const IO*)a.Bm + b * a.B_sb + g * a.B_sg);
-    C[r] = cols((const IO*)a.Cm + b * a.C_sb + g * a.C_sg);
-    len[r] = a.len ? a.len[b] : 1;
+    const int64_t k = r < left ? r : 0;
+    h[r] = h0 ? four(h0 + k * a.Dm * a.N) : make_float4(0.f, 0.f, 0.f, 0.f);
+    B[r] = cols(pB + k * a.B_sb);
+    C[r] = cols(pC + k * a.C_sb);
   }
+  IO ru[RPL], rd[RPL], rz[RPL];
+  int len[RPL];
+#pragma unroll
+  for (int j = 0; j < RPL; ++j) {
+    const int64_t b = b0 + (k0 + j < left ? k0 + j : 0);
+    ru[j] = ((const IO*)a.u)[b * a.u_sb + dd];
+    rd[j] = ((const IO*)a.delta)[b * a.d_sb + dd];
+    rz[j] = a.z ? ((const IO*)a.z)[b * a.z_sb + dd] : ru[j];
+    len[j] = a.len ? a.len[b] : 1;
+  }
+  float u[RPL], x[RPL], xu[RPL];
+#pragma unroll
+  for (int j = 0; j < RPL; ++j) {
+    u[j] = to_f(ru[j]);
+    x[j] = to_f(rd[j]) + bias;
+    if (a.softplus) x[j] = softplus(x[j]);
+    xu[j] = x[j] * u[j];
+  }
+  const float Av[4] = {log2_decay(A.x), log2_decay(A.y), log2_decay(A.z), log2_decay(A.w)};
+  float y[R];
+  float* ho = a.hT + (b0 * a.Dm + d) * a.N + n4;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int64_t b = (int64_t)blockIdx.y * R + r;
-    const bool live = len[r] > 0;
-    float hv[4] = {h[r].x, h[r].y, h[r].z, h[r].w}, y = 0.f;
-    const float Av[4] = {log2_decay(A.x), log2_decay(A.y), log2_decay(A.z), log2_decay(A.w)}, u = live ? to_f(du[r]) : 0.f;
-    float x = to_f(dd_[r]) + bias;
-    if (a.softplus) x = softplus(x);
-    if (!live) x = 0.f;
-    const float xu = x * u;
+    const float xr = __shfl_sync(0xffffffffu, x[r % RPL], r / RPL, LPC), xur = __shfl_sync(0xffffffffu, xu[r % RPL], r / RPL, LPC);
+    const bool live = !a.len || __shfl_sync(0xffffffffu, len[r % RPL], r / RPL, LPC) > 0;
+    float hv[4] = {h[r].x, h[r].y, h[r].z, h[r].w};
+    y[r] = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float Bv = live ? to_f(B[r].v[i]) : 0.f, Cv = live ? to_f(C[r].v[i]) : 0.f;
-      hv[i] = fmaf(ex2(Av[i] * x), hv[i], xu * Bv);
-      if (V4 ? on : n4 + i < a.N) y = fmaf(Cv, hv[i], y);
+      const float v = fmaf(ex2(Av[i] * xr), hv[i], xur * to_f(B[r].v[i]));
+      if (live) hv[i] = v;
+      if (V4 ? on : n4 + i < a.N) y[r] = fmaf(to_f(C[r].v[i]), hv[i], y[r]);
     }
+    if (d < a.Dm && r < left) {
+      float* o = ho + (int64_t)r * a.Dm * a.N;
+      if (V4) {
+        if (on) *reinterpret_cast<float4*>(o) = make_float4(hv[0], hv[1], hv[2], hv[3]);
+      } else {
 #pragma unroll
-    for (int o = LPC / 2; o >= 1; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (d >= a.Dm || b >= a.Bsz) continue;
-    float* ho = a.hT + (b * a.Dm + d) * a.N + n4;
-    if (V4) {
-      if (on) *reinterpret_cast<float4*>(ho) = make_float4(hv[0], hv[1], hv[2], hv[3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n4 + i < a.N) ho[i] = hv[i];
-    }
-    if (n4 == 0) {
-      y = fmaf(skip, u, y);
-      if (a.z) {
-        const float zz = to_f(dz[r]);
-        y *= zz * sigmoid(zz);
+        for (int i = 0; i < 4; ++i)
+          if (n4 + i < a.N) o[i] = hv[i];
       }
-      from_f(((IO*)a.out)[b * a.Dm + d], live ? y : 0.f);
     }
+  }
+  reduce_part<R, L, 1>(y, threadIdx.x & 31);
+#pragma unroll
+  for (int o = L; o < LPC; o <<= 1)
+#pragma unroll
+    for (int j = 0; j < RPL; ++j) y[j] += __shfl_xor_sync(0xffffffffu, y[j], o);
+  if (l >= L || d >= a.Dm) return;
+#pragma unroll
+  for (int j = 0; j < RPL; ++j) {
+    if (k0 + j >= left) continue;
+    float v = fmaf(skip, u[j], y[j]);
+    if (a.z) {
+      const float z = to_f(rz[j]);
+      v *= z * sigmoid(z);
+    }
+    from_f(((IO*)a.out)[(b0 + k0 + j) * a.Dm + d], len[j] > 0 ? v : 0.f);
   }
 }
 
