@@ -41,7 +41,7 @@ struct ConvArgs {
   const int* len;
   void *y, *final_state, *dx, *d_init;
   float* part;  // [B * ygrid, C, K + 1]: dw, dbias of a CTA's steps
-  int64_t T, C;
+  int64_t T, C, rows;
   int run, ygrid, silu, vec;  // steps per thread; CTAs along the time axis
 };
 
@@ -177,15 +177,16 @@ __global__ void __launch_bounds__(32 * kConvWarps) k_causal_conv_fwd(const ConvA
   for (; t < q.n; ++t) store<IO, W>(y + t * a.C, zeros<IO, W>(), q.nc, q.fast);
 }
 
-// One step (T = 1): a thread reads its channels' K - 1 carried inputs and the new one once, all in flight together, and
-// writes y and the shifted state. FAST: whole vectors. grid (channel blocks, batch).
+// One step (T = 1): a thread reads its channels' taps, and of R batch rows the K - 1 carried inputs and the new one, all in
+// flight together, and writes y and the shifted states. FAST: whole vectors. grid (channel blocks, row blocks).
 constexpr int kConvStepThr = 128;
-template <int K, class IO, int W, bool FAST>
+template <int K, class IO, int W, int R, bool FAST>
 __global__ void __launch_bounds__(kConvStepThr) k_causal_conv_step(const ConvArgs a) {
   constexpr int P = W / 2;
-  const int64_t b = blockIdx.y, c = ((int64_t)blockIdx.x * kConvStepThr + threadIdx.x) * W;
+  const int64_t b0 = (int64_t)blockIdx.y * R, c = ((int64_t)blockIdx.x * kConvStepThr + threadIdx.x) * W;
   if (c >= a.C) return;
   const int nc = a.C - c < W ? (int)(a.C - c) : W;
+  const int left = a.rows - b0 < R ? (int)(a.rows - b0) : R;
   auto raw = [&](const IO* p) {
     if (FAST) return *reinterpret_cast<const Vec<IO, W>*>(p);
     return ss::load_row<IO, W>(p, 0, nc, 0);
@@ -194,33 +195,53 @@ __global__ void __launch_bounds__(kConvStepThr) k_causal_conv_step(const ConvArg
     if (FAST) *reinterpret_cast<Vec<IO, W>*>(p) = r;
     else ss::store_row<IO, W>(p, 0, nc, 0, r);
   };
-  Vec<IO, W> v[K];
+  const int64_t state = (K - 1) * a.C;
+  const IO* init = a.init ? (const IO*)a.init + b0 * state + c : nullptr;
+  const IO* x = (const IO*)a.x + b0 * a.x_sb + c;
+  Vec<IO, W> v[R][K];
+  int len[R];
 #pragma unroll
-  for (int j = 0; j < K - 1; ++j)
-    v[j] = a.init ? raw((const IO*)a.init + (b * (K - 1) + j) * a.C + c) : ss::zero_row<IO, W>();
-  v[K - 1] = raw((const IO*)a.x + b * a.x_sb + c);
+  for (int r = 0; r < R; ++r) {
+    const int64_t k = r < left ? r : 0;  // rows that exist
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) v[r][j] = init ? raw(init + k * state + j * a.C) : ss::zero_row<IO, W>();
+    v[r][K - 1] = raw(x + k * a.x_sb);
+    len[r] = a.len ? a.len[b0 + k] : 1;
+  }
   float w[W][K], bias[W];
+  if (FAST && W * K % 4 == 0) {  // the channels' taps lie side by side (alignment: `vec` asks for 16 bytes of w)
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    const int64_t k = FAST || i < nc ? c + i : c;
-    bias[i] = a.bias ? a.bias[k] : 0.f;
+    for (int i = 0; i < W * K / 4 * 4; i += 4) {
+      const float4 t = *reinterpret_cast<const float4*>(a.w + c * K + i);
+      w[i / K][i % K] = t.x, w[(i + 1) / K][(i + 1) % K] = t.y, w[(i + 2) / K][(i + 2) % K] = t.z, w[(i + 3) / K][(i + 3) % K] = t.w;
+    }
+  } else {
 #pragma unroll
-    for (int j = 0; j < K; ++j) w[i][j] = a.w[k * K + j];
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+      for (int j = 0; j < K; ++j) w[i][j] = a.w[(FAST || i < nc ? c + i : c) * K + j];
   }
-  const bool live = row_len(a.len, (int)b, 1) > 0;
-  IO* f = (IO*)a.final_state + b * (K - 1) * a.C + c;
 #pragma unroll
-  for (int j = 0; j < K - 1; ++j) put(f + j * a.C, live ? v[j + 1] : v[j]);
-  Vec<IO, W> o;
+  for (int i = 0; i < W; ++i) bias[i] = a.bias ? a.bias[FAST || i < nc ? c + i : c] : 0.f;
+  IO* f = (IO*)a.final_state + b0 * state + c;
+  IO* y = (IO*)a.y + b0 * a.C + c;
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    f2 s = pk(bias[2 * i], bias[2 * i + 1]);
+  for (int r = 0; r < R; ++r) {
+    if (r >= left) break;
+    const bool live = len[r] > 0;
 #pragma unroll
-    for (int j = 0; j < K; ++j) s = fma2(pk(w[2 * i][j], w[2 * i + 1][j]), ld2(&v[j].v[2 * i]), s);
-    if (a.silu) s = mul2(s, sigmoid_2(s));
-    st2(&o.v[2 * i], live ? s : 0);
+    for (int j = 0; j < K - 1; ++j) put(f + r * state + j * a.C, live ? v[r][j + 1] : v[r][j]);
+    Vec<IO, W> o;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      f2 s = pk(bias[2 * i], bias[2 * i + 1]);
+#pragma unroll
+      for (int j = 0; j < K; ++j) s = fma2(pk(w[2 * i][j], w[2 * i + 1][j]), ld2(&v[r][j].v[2 * i]), s);
+      if (a.silu) s = mul2(s, sigmoid_2(s));
+      st2(&o.v[2 * i], live ? s : 0);
+    }
+    put(y + r * a.C, o);
   }
-  put((IO*)a.y + b * a.C + c, o);
 }
 
 template <int K, class IO, int W>
