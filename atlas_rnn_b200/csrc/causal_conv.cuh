@@ -5,6 +5,8 @@
 // run of steps, its taps and window in registers; a warp's lanes take neighbouring channel groups, so each load is a
 // contiguous row segment, kConvU steps of them in flight. HBM-bound: the forward reads x once (plus K - 1 steps a run) and writes
 // y; the backward reads x and dy, recomputes pre for the activation's slope and writes dx:
+// B 4, T 8192, C 1536, K 4, bf16: forward 51 us (3.9 TB/s), backward 100 (3.0 TB/s), both waiting for loads with the warps
+// that their registers leave. Results are rounded to the rows' type once, when they are written.
 //   dp_t = dy_t act'(pre_t),  dx_s = sum_j w[j] dp_{s + K-1 - j},  dw[j] = sum_t dp_t x[t + j - (K-1)],  dbias = sum_t dp_t.
 // Weight gradients: per-thread sums over the run, added over the CTA's four runs in shared memory, one record a CTA,
 // records added in order by k_causal_conv_dw (no atomics: the same inputs give the same bits).

@@ -21,7 +21,7 @@ void configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& at, int64_t rows, i
   cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = kBytes<IO, NT>;
   cfg.stream = st;
-  cfg.attrs = &at, cfg.numAttrs = C > 1;
+  cfg.attrs = &at, cfg.numAttrs = C > 1;  // a plain launch for rows of one CTA
 }
 
 // Clusters of C CTAs that run at a time on the current device. Below 148 / C: a cluster stays within a group of SMs.
