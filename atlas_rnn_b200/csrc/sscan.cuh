@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kCarryThr) k_sscan_carry(const ScanArgs a) {
 // ---- one token ------------------------------------------------------------
 // T = 1 without a backward: a thread takes 4 neighbouring states (one 16-byte read and write of the state, which is the
 // traffic) of R batch rows, whose loads are all in flight together; LPC = NP / 4 lanes a channel. A, D and bias are read
-// once for the R rows. What a row needs once a channel (dt, the gate, the output) is done by one of the channel's lanes, R
+// once for the R rows (1 or 4). What a row needs once a channel (dt, the gate, the output) is done by one of the channel's lanes, R
 // rows by as many lanes. grid (channel blocks, row blocks).
 constexpr int kStepThr = 128;
 // V4: 16-byte accesses to A and the states, 4-element ones to B and C (N a multiple of 4)
@@ -512,9 +512,14 @@ __global__ void __launch_bounds__(kStepThr) k_sscan_step(const ScanArgs a) {
       }
     }
   }
+  // lanes 2 apart first, then 1, then 4 and more, whatever R is: a row's result does not depend on the rows beside it
   reduce_part<R, L, 1>(y, threadIdx.x & 31);
+  if (R == 1) {
 #pragma unroll
-  for (int o = L; o < LPC; o <<= 1)
+    for (int o = LPC < 4 ? LPC / 2 : 2; o > 0; o >>= 1) y[0] += __shfl_xor_sync(0xffffffffu, y[0], o);
+  }
+#pragma unroll
+  for (int o = R == 1 ? 4 : L; o < LPC; o <<= 1)
 #pragma unroll
     for (int j = 0; j < RPL; ++j) y[j] += __shfl_xor_sync(0xffffffffu, y[j], o);
   if (l >= L || d >= a.Dm) return;

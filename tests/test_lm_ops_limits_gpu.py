@@ -228,3 +228,52 @@ def test_extreme_temperatures(native_lib):
     for t in (1e-29, 1e-6, 1e30):
         assert torch.equal(sample_tokens(x, u, temperature=t).cpu(), sample_reference(x, u, temperature=t))
     assert torch.equal(sample_tokens(x, u, temperature=1e-40), x.argmax(-1))
+
+
+@pytest.mark.parametrize("N,G,z,dtype", [(5, 1, True, torch.float32), (8, 3, False, torch.bfloat16), (16, 1, True, torch.bfloat16),
+                                         (17, 2, True, torch.float32), (32, 1, False, torch.float32),
+                                         (64, 1, True, torch.bfloat16)])
+def test_one_token_for_many_rows(native_lib, N, G, z, dtype):
+    """Several rows a thread, the last ones fewer; rows without a step hold NaN."""
+    B, D = 1190 + 3, 6
+    g = torch.Generator().manual_seed(N)
+    x = make(B, 1, D, G, N, dtype, z=z)
+    x["lengths"] = (torch.rand(B, generator=g) < 0.8).int().cuda()
+    _, ref, ref_h = reference(x)
+    dead = x["lengths"] == 0
+    for k in ("u", "delta", "B", "C", "z"):
+        if x[k] is not None:
+            x[k][dead] = float("nan")
+    with torch.no_grad():
+        out, h = call(x)
+    assert rel_l2(out.float(), ref) <= tol(1, dtype) and rel_l2(h, ref_h) <= tol(1, torch.float32)
+    assert (out[dead] == 0).all() and torch.equal(h[dead], x["initial_state"][dead])
+    x["lengths"] = None
+    x = {k: v if v is None else v[~dead] if v.shape[0] == B else v for k, v in x.items()}
+    with torch.no_grad():
+        again = call(x)
+    assert torch.equal(again[0], out[~dead]) and torch.equal(again[1], h[~dead])
+
+
+@pytest.mark.parametrize("C,K,dtype", [(6, 2, torch.float32), (1028, 3, torch.bfloat16), (64, 4, torch.bfloat16),
+                                       (7, 5, torch.float32), (130, 6, torch.float32), (9, 7, torch.bfloat16),
+                                       (36, 8, torch.float32)])
+def test_one_convolution_step_for_many_rows(native_lib, C, K, dtype):
+    from atlas_rnn_b200 import causal_conv1d
+    from tests.test_selective_scan_gpu import conv_reference
+    B = 303
+    rn = gen(C)
+    x, w, bias, init = rn(B, 1, C).to(dtype), rn(C, K), rn(C), rn(B, K - 1, C).to(dtype)
+    lengths = (torch.rand(B, device="cuda") < 0.8).int()
+    _, ref, ref_f = conv_reference(x, w, bias, True, init, lengths)
+    x[lengths == 0] = float("nan")
+    y, final = causal_conv1d(x, w, bias, activation="silu", initial_state=init, lengths=lengths)
+    # K products and the activation in fp32, as for longer rows: 2^-18, and half a step of bf16
+    assert rel_l2(y.float(), ref) <= 2.0 ** -18 + (2.0 ** -8 if dtype == torch.bfloat16 else 0.0)
+    assert torch.equal(final.double().cpu(), ref_f)
+    # taps at any alignment, few rows
+    shifted = torch.empty(C * K + 1, device="cuda")[1:].view(C, K).copy_(w)
+    some = slice(0, 5)
+    for v in (w, shifted):
+        o, f = causal_conv1d(x[some], v, bias, activation="silu", initial_state=init[some], lengths=lengths[some])
+        assert torch.equal(o, y[some]) and torch.equal(f, final[some])
