@@ -20,7 +20,7 @@ bool pack(const AtlasDistill* p, DistillArgs& a, int& C) {
     return false;
   a.logits = p->logits, a.stride = p->stride, a.values = p->values, a.indices = p->indices;
   a.loss = p->loss, a.valid = p->valid, a.stats = p->stats, a.dloss = p->dloss, a.dlogits = p->dlogits;
-  a.V = (int)p->V, a.K = (int)p->K, a.tau = p->temperature;
+  a.V = (int)p->V, a.K = (int)p->K, a.rows = (int)p->rows, a.tau = p->temperature;
   // a row's CTAs: one where the rows fill the machine, else up to 8 with at least 4096 tokens each
   C = 8;
   while (C > 1 && (p->rows * C > 4 * sm_count() || p->V / C < 4096)) C /= 2;
@@ -28,8 +28,15 @@ bool pack(const AtlasDistill* p, DistillArgs& a, int& C) {
   return true;
 }
 
+bool short_rows(const DistillArgs& a) { return a.V <= kShortV && a.K <= kShortK; }
+
 template <class IO, int NT>
 int fwd(const DistillArgs& a, int64_t rows, int C, cudaStream_t st) {
+  if (short_rows(a)) {
+    LAUNCH_T(KID_DISTILL_FWD, (k_distill_fwd<IO, 32, kShortRows>), dim3((unsigned)((rows + kShortRows - 1) / kShortRows)),
+             32 * kShortRows, 0, st, a);
+    return ATLAS_OK;
+  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at = {};
   at.id = cudaLaunchAttributeClusterDimension;
@@ -39,14 +46,19 @@ int fwd(const DistillArgs& a, int64_t rows, int C, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = &at, cfg.numAttrs = C > 1;  // plain launches where they do: CTAs start faster (8192 x 32000: 103 us, not 115)
   const int slot = prof_begin(KID_DISTILL_FWD, st);
-  if (cudaLaunchKernelEx(&cfg, k_distill_fwd<IO, NT>, a) != cudaSuccess) return ATLAS_ERR_LAUNCH;
+  if (cudaLaunchKernelEx(&cfg, k_distill_fwd<IO, NT, 1>, a) != cudaSuccess) return ATLAS_ERR_LAUNCH;
   LAUNCH_CHECK();
   prof_end(slot, st);
   return ATLAS_OK;
 }
 template <class IO, int NT>
 int bwd(const DistillArgs& a, int64_t rows, int C, cudaStream_t st) {
-  LAUNCH_T(KID_DISTILL_BWD, (k_distill_bwd<IO, NT>), dim3((unsigned)(rows * C)), NT, 0, st, a, C);
+  if (short_rows(a)) {
+    LAUNCH_T(KID_DISTILL_BWD, (k_distill_bwd<IO, 32, kShortRows>), dim3((unsigned)((rows + kShortRows - 1) / kShortRows)),
+             32 * kShortRows, 0, st, a, 1);
+    return ATLAS_OK;
+  }
+  LAUNCH_T(KID_DISTILL_BWD, (k_distill_bwd<IO, NT, 1>), dim3((unsigned)(rows * C)), NT, 0, st, a, C);
   return ATLAS_OK;
 }
 

@@ -19,6 +19,9 @@ namespace dst {
 namespace cg = cooperative_groups;
 constexpr int kMaxK = 1024;
 constexpr int kMarks = 512;  // words of a bitmap of tokens, by their low bits
+// Short rows of few entries: a warp a row, 4 rows a CTA, since the start of a CTA costs more than such a row (32768 x 256,
+// bf16, 20 entries: forward 25 us, backward 29; a CTA a row 50 and 67).
+constexpr int kShortV = 1024, kShortK = 128, kShortRows = 4;
 
 struct DistillArgs {
   const void* logits;
@@ -31,6 +34,7 @@ struct DistillArgs {
   const float* dloss;
   void* dlogits;  // [rows, V]
   int V, K, split;
+  int rows;
   float tau;
 };
 
@@ -71,15 +75,17 @@ __device__ __forceinline__ float weight(float v, float top, float c) {
   return v == top ? 1.f : exp2f((v - top) * c);
 }
 
-// grid rows x cluster
-template <class IO, int NT>
-__global__ void __launch_bounds__(NT) k_distill_fwd(const DistillArgs a) {
+// grid rows x cluster; NT threads a row, RPC rows a CTA (then one warp a row)
+template <class IO, int NT, int RPC>
+__global__ void __launch_bounds__(NT * RPC) k_distill_fwd(const DistillArgs a) {
   constexpr int E = 16 / (int)sizeof(IO), NW = NT / 32, U = 4;
+  static_assert(RPC == 1 || NT == 32, "rows of a CTA share no barrier");
   __shared__ float s_m[NW], s_s[NW], s_cm[8], s_cs[8];
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int64_t row = blockIdx.x / C;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t row = RPC > 1 ? (int64_t)blockIdx.x * RPC + threadIdx.x / NT : blockIdx.x / C;
+  const int tid = threadIdx.x % NT, lane = tid & 31, warp = tid >> 5;
+  if (RPC > 1 && row >= a.rows) return;
   if (C > 1) cluster.barrier_arrive();  // waited for before another CTA's memory is touched
   const float c = ss::kLog2e / a.tau;
   const IO* x = (const IO*)a.logits + row * a.stride;
@@ -131,11 +137,14 @@ __global__ void __launch_bounds__(NT) k_distill_fwd(const DistillArgs a) {
   // over the block, then the cluster; sums of empty parts weigh 2^-inf = 0
   auto join = [&](float m0, float s0, float m1) { return m0 > -INFINITY ? s0 * ss::ex2((m0 - m1) * c) : s0; };
   const float wm = warp_reduce(m, fmax_op), ws = warp_reduce(join(m, s, wm), add_op);
-  if (lane == 0) s_m[warp] = wm, s_s[warp] = ws;
-  __syncthreads();
-  if (warp != 0 && C == 1) return;  // the first warp finishes the row: no further block barriers
-  const float lm = lane < NW ? s_m[lane] : -INFINITY, lsum = lane < NW ? s_s[lane] : 0.f;
-  float bm = warp_reduce(lm, fmax_op), bs = warp_reduce(join(lm, lsum, bm), add_op);
+  float bm = wm, bs = ws;
+  if (NW > 1) {
+    if (lane == 0) s_m[warp] = wm, s_s[warp] = ws;
+    __syncthreads();
+    if (warp != 0 && C == 1) return;  // the first warp finishes the row: no further block barriers
+    const float lm = lane < NW ? s_m[lane] : -INFINITY, lsum = lane < NW ? s_s[lane] : 0.f;
+    bm = warp_reduce(lm, fmax_op), bs = warp_reduce(join(lm, lsum, bm), add_op);
+  }
   if (C > 1) {
     cluster.barrier_wait();
     if (tid == 0) {
@@ -186,27 +195,37 @@ __global__ void __launch_bounds__(NT) k_distill_fwd(const DistillArgs a) {
 // the entries' low bits (seen, seen again) clear most of being repeated, and a warp looks together through all entries for
 // each of the others (8192 x 32000, bf16: 172 us with 20 entries, 217 with 256, 399 with 1024; with every entry looking
 // through all of them 172, 238 and 1500).
-template <class IO, int NT>
-__global__ void __launch_bounds__(NT) k_distill_bwd(const DistillArgs a, int C) {
-  constexpr int E = 16 / (int)sizeof(IO), U = 4;
-  __shared__ float s_p[kMaxK];
-  __shared__ int s_t[kMaxK];
-  __shared__ unsigned s_seen[kMarks], s_again[kMarks];
-  const int64_t row = blockIdx.x / C;
-  const int rank = (int)(blockIdx.x - row * C), tid = threadIdx.x;
+template <class IO, int NT, int RPC>
+__global__ void __launch_bounds__(NT * RPC) k_distill_bwd(const DistillArgs a, int C) {
+  static_assert(RPC == 1 || NT == 32, "rows of a CTA share no barrier");
+  constexpr int E = 16 / (int)sizeof(IO), U = 4, KM = RPC > 1 ? kShortK : kMaxK, MARKS = RPC > 1 ? kShortV / 32 : kMarks;
+  __shared__ float s_p_[RPC][KM];
+  __shared__ int s_t_[RPC][KM];
+  __shared__ unsigned s_seen_[RPC][MARKS], s_again_[RPC][MARKS];
+  const int tid = threadIdx.x % NT, sub = threadIdx.x / NT;
+  const int64_t row = RPC > 1 ? (int64_t)blockIdx.x * RPC + sub : blockIdx.x / C;
+  if (RPC > 1 && row >= a.rows) return;
+  const int rank = RPC > 1 ? 0 : (int)(blockIdx.x - row * C);
+  float* s_p = s_p_[sub];
+  int* s_t = s_t_[sub];
+  unsigned *s_seen = s_seen_[sub], *s_again = s_again_[sub];
+  auto sync = [] {
+    if (RPC > 1) __syncwarp();
+    else __syncthreads();
+  };
   const int lo = rank * a.split, n = a.V - lo < a.split ? (a.V - lo < 0 ? 0 : a.V - lo) : a.split;
   const float4 st = *reinterpret_cast<const float4*>(a.stats + row * 4);
   const float c = ss::kLog2e / a.tau, g = a.dloss[row] * a.tau;
   const bool some = st.w > 0.f;
   const IO* x = (const IO*)a.logits + row * a.stride;
   IO* o = (IO*)a.dlogits + row * a.V;
-  for (int i = tid; i < kMarks; i += NT) s_seen[i] = s_again[i] = 0;
-  __syncthreads();
+  for (int i = tid; i < MARKS; i += NT) s_seen[i] = s_again[i] = 0;
+  sync();
   for (int k = tid; k < a.K; k += NT) {
     int64_t t;
     const float v = entry(a, row, k, t);
     if (v > -INFINITY) {
-      const unsigned w = (unsigned)t / 32 % kMarks, bit = 1u << (t & 31);
+      const unsigned w = (unsigned)t / 32 % MARKS, bit = 1u << (t & 31);
       if (atomicOr(&s_seen[w], bit) & bit) atomicOr(&s_again[w], bit);
     }
     s_t[k] = v > -INFINITY ? (int)t : -1;
@@ -239,13 +258,13 @@ __global__ void __launch_bounds__(NT) k_distill_bwd(const DistillArgs a, int C) 
     const int at = i < head ? i : i + nv * E;
     ss::from_f(ol[at], grad(ss::to_f(xl[at])));
   }
-  __syncthreads();  // the entries' own values go over those above; equal tokens write the same sum
+  sync();  // the entries' own values go over those above; equal tokens write the same sum
   const int lane = tid & 31;
   for (int k = tid; k - lane < a.K; k += NT) {
     const int t = k < a.K ? s_t[k] : -1;
     const bool mine = t >= lo && t < lo + n;
     float p = mine ? s_p[k] : 0.f;
-    unsigned again = __ballot_sync(0xffffffffu, mine && s_again[(unsigned)t / 32 % kMarks] >> (t & 31) & 1);
+    unsigned again = __ballot_sync(0xffffffffu, mine && s_again[(unsigned)t / 32 % MARKS] >> (t & 31) & 1);
     for (; again; again &= again - 1) {
       const int l = __ffs(again) - 1, tl = __shfl_sync(0xffffffffu, t, l);
       float q = 0.f;
