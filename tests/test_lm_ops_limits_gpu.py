@@ -277,3 +277,47 @@ def test_one_convolution_step_for_many_rows(native_lib, C, K, dtype):
     for v in (w, shifted):
         o, f = causal_conv1d(x[some], v, bias, activation="silu", initial_state=init[some], lengths=lengths[some])
         assert torch.equal(o, y[some]) and torch.equal(f, final[some])
+
+
+@pytest.mark.parametrize("K,dtype,C", [(2, torch.bfloat16, 8192), (3, torch.float32, 8192), (4, torch.bfloat16, 8192),
+                                       (4, torch.float32, 8190), (4, torch.bfloat16, 8191), (8, torch.bfloat16, 8192)])
+def test_convolution_of_long_runs(native_lib, K, dtype, C):
+    """Sizes that fill the machine, where a thread walks its longest runs, against float64 on the GPU."""
+    from atlas_rnn_b200 import causal_conv1d
+    B, T = 2, 4133
+    rn = gen(K)
+    x, w, bias = rn(B, T, C).to(dtype).requires_grad_(True), rn(C, K).requires_grad_(True), rn(C).requires_grad_(True)
+    init = rn(B, K - 1, C).to(dtype).requires_grad_(True)
+    lengths = torch.tensor([T, 1030], device="cuda")
+    dy, df = rn(B, T, C).to(dtype), rn(B, K - 1, C).to(dtype)
+    y, final = causal_conv1d(x, w, bias, activation="silu", initial_state=init, lengths=lengths)
+    got = torch.autograd.grad((y, final), (x, w, bias, init), (dy, df))
+    leaf = [t.detach().double().requires_grad_(True) for t in (x, w, bias, init)]
+    full = torch.cat([leaf[3], leaf[0]], 1)
+    ref = torch.nn.functional.silu(leaf[2] + sum(full[:, j:j + T] * leaf[1][:, j] for j in range(K)))
+    ref = ref * (torch.arange(T, device="cuda")[:, None] < lengths[:, None, None])
+    ref_f = torch.stack([full[b, e:e + K - 1] for b, e in enumerate(lengths.tolist())])
+    want = torch.autograd.grad((ref, ref_f), leaf, (dy.double(), df.double()))
+    # as for short rows: 2^-18, half a step of bf16; the parameters' sums of 5163 terms in fp32 by runs, records and CTAs keep
+    # to 2^-18 of the sum of their sizes, against a sum that cancels to its square root (1/72 of it): 2^-12
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+    rel = lambda a, b: ((a.double() - b).norm() / b.norm()).item()
+    assert rel(y, ref) <= 2.0 ** -18 + half and torch.equal(final.double(), ref_f)
+    for name, g, r in zip(("x", "w", "bias", "init"), got, want):
+        assert rel(g, r) <= (2.0 ** -12 if name in ("w", "bias") else 2.0 ** -18 + half), (name, rel(g, r))
+
+
+def test_cuts_of_the_time_axis_agree(native_lib):
+    """The library's own cut at a size that fills the machine, short and long pieces, and none."""
+    x = make(3, 2500, 1536, 1, 16, lengths=(2500, 1111, 0))
+    leaves = [x[k].requires_grad_(True) for k in NAMES]
+    rn = gen(11)
+    w, wh = rn(3, 2500, 1536), rn(3, 1536, 16)
+    runs = []
+    for chunk in (2528, 0, 64, 1024):  # the first: one piece
+        out, h = call(x, chunk=chunk)
+        runs.append([out, h, *torch.autograd.grad((out, h), leaves, (w, wh))])
+    for r in runs[1:]:
+        for name, a, b in zip(("out", "state", *NAMES), r, runs[0]):
+            # either side is within tol of the exact result (twice that for gradients, as in the tests of short sequences)
+            assert rel_l2(a, b) <= 4 * tol(2500, torch.float32), (name, rel_l2(a, b))
