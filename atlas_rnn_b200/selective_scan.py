@@ -16,6 +16,7 @@ import struct
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -87,6 +88,12 @@ def _wants_grad(*tensors) -> bool:
     return any(t is not None and t.requires_grad for t in tensors)
 
 
+def _through_autograd(keep: bool) -> bool:
+    """Whether a call goes through its autograd function: for a backward pass, and inside a dual level, where the function
+    refuses inputs with a tangent (a call past it would drop the tangent). Else the call itself saves the detour's time."""
+    return keep or forward_ad._current_level >= 0
+
+
 def _run(what: str, fn, device, *args):
     """fn(*args, current stream of device) with ``device`` current: kernels launch on the current device."""
     index = device.index
@@ -155,10 +162,10 @@ class _Scan:
 
 class SelectiveScanFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, u, delta, A, B, C, D, z, bias, h0, lengths, softplus, chunk):
+    def forward(ctx, u, delta, A, B, C, D, z, bias, h0, lengths, softplus, chunk, keep):
         ctx.set_materialize_grads(False)
         s = _Scan(u, delta, A, B, C, D, z, bias, h0, lengths, softplus, chunk)
-        out, hT, saved = s.forward(keep=True)
+        out, hT, saved = s.forward(keep)
         ctx.save_for_backward(u, delta, A, B, C, D, z, bias, h0, lengths, saved)
         ctx.softplus, ctx.chunk = softplus, chunk
         return out, hT
@@ -182,7 +189,7 @@ class SelectiveScanFn(torch.autograd.Function):
         packed = s.pack(saved=saved, scratch=scratch, dout=dout, dhT=dhT, du=du, ddelta=ddelta, dz=dz, dB=dB, dC=dC,
                         dA=dA, dD=dD, dbias=dbias, dh0=dh0)
         _run("selective_scan backward", _lib.lib().atlas_sscan_backward, dev, packed)
-        return du, ddelta, dA, dB, dC, dD, dz, dbias, dh0, None, None, None
+        return du, ddelta, dA, dB, dC, dD, dz, dbias, dh0, None, None, None, None
 
 
 def _no_steps(u: Tensor, N: int, h0: Tensor | None):
@@ -244,8 +251,9 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D:
         return _no_steps(u, n, h0)
     u, delta, B, C = _rows(u), _rows(delta), _rows(B), _rows(C)
     z = None if z is None else _rows(z)
-    if _wants_grad(u, delta, A, B, C, D, z, bias, h0):
-        return SelectiveScanFn.apply(u, delta, A, B, C, D, z, bias, h0, lengths, bool(delta_softplus), chunk)
+    keep = _wants_grad(u, delta, A, B, C, D, z, bias, h0)
+    if _through_autograd(keep):
+        return SelectiveScanFn.apply(u, delta, A, B, C, D, z, bias, h0, lengths, bool(delta_softplus), chunk, keep)
     out, hT, _ = _Scan(u, delta, A, B, C, D, z, bias, h0, lengths, bool(delta_softplus), chunk).forward(keep=False)
     return out, hT
 
@@ -331,6 +339,6 @@ def causal_conv1d(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, acti
         final = x.new_zeros(B, K - 1, C) if initial_state is None else initial_state.clone()
         return torch.empty_like(x, memory_format=torch.contiguous_format), final
     x = _rows(x)
-    if _wants_grad(x, w, bias, initial_state):
+    if _through_autograd(_wants_grad(x, w, bias, initial_state)):
         return CausalConv1dFn.apply(x, w, bias, initial_state, lengths, silu)
     return _conv_forward(x, w, bias, initial_state, lengths, silu)
