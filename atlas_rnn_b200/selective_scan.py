@@ -16,10 +16,10 @@ import struct
 
 import torch
 from torch import Tensor
-from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+from .ops import _has_tangent
 
 MAX_STATE = 64     # states per channel
 MAX_CONV_K = 8     # taps
@@ -82,16 +82,10 @@ def _lengths(what: str, lengths, batch: int, device) -> Tensor | None:
         else lengths.contiguous()
 
 
-def _wants_grad(*tensors) -> bool:
-    if not torch.is_grad_enabled():
-        return False
-    return any(t is not None and t.requires_grad for t in tensors)
-
-
-def _through_autograd(keep: bool) -> bool:
-    """Whether a call goes through its autograd function: for a backward pass, and inside a dual level, where the function
-    refuses inputs with a tangent (a call past it would drop the tangent). Else the call itself saves the detour's time."""
-    return keep or forward_ad._current_level >= 0
+def _through_autograd(*tensors) -> bool:
+    """Whether a call goes through its autograd function: for a backward pass, and with a forward-mode tangent, which the
+    function refuses (a call past it would drop the tangent). Else the call itself saves the detour's time."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or _has_tangent(*tensors)
 
 
 def _run(what: str, fn, device, *args):
@@ -149,6 +143,9 @@ class _Scan:
         """(out, final state, kept states or None)."""
         u = self.u
         dev = u.device
+        if u.numel() == 0:  # nothing to walk (no rows or no steps): the state passes through
+            hT = u.new_zeros(u.shape[0], u.shape[2], self.B.shape[3], dtype=torch.float32) if self.h0 is None else self.h0.clone()
+            return torch.empty_like(u, memory_format=torch.contiguous_format), hT, None
         out = torch.empty(u.shape, dtype=u.dtype, device=dev)
         hT = torch.empty(u.shape[0], u.shape[2], self.B.shape[3], dtype=torch.float32, device=dev)
         saved = scratch = None
@@ -160,65 +157,8 @@ class _Scan:
         return out, hT, saved
 
 
-class SelectiveScanFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, u, delta, A, B, C, D, z, bias, h0, lengths, softplus, chunk, keep):
-        ctx.set_materialize_grads(False)
-        s = _Scan(u, delta, A, B, C, D, z, bias, h0, lengths, softplus, chunk)
-        out, hT, saved = s.forward(keep)
-        ctx.save_for_backward(u, delta, A, B, C, D, z, bias, h0, lengths, saved)
-        ctx.softplus, ctx.chunk = softplus, chunk
-        return out, hT
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout, dhT):
-        u, delta, A, B, C, D, z, bias, h0, lengths, saved = ctx.saved_tensors
-        need = ctx.needs_input_grad  # (u, delta, A, B, C, D, z, bias, h0, ...)
-        s = _Scan(u, delta, A, B, C, D, z, bias, h0, lengths, ctx.softplus, ctx.chunk)
-        dev = u.device
-        dout = torch.zeros(u.shape, dtype=u.dtype, device=dev) if dout is None else _rows(dout)
-        dhT = None if dhT is None else dhT.contiguous()
-        rows = lambda: torch.empty(u.shape, dtype=u.dtype, device=dev)
-        du, ddelta, dz = rows(), rows(), rows() if z is not None else None
-        dB = torch.empty(B.shape, dtype=u.dtype, device=dev) if need[3] or need[4] else None
-        dC = torch.empty(C.shape, dtype=u.dtype, device=dev) if need[3] or need[4] else None
-        f32 = lambda t, flag: torch.empty(t.shape, dtype=torch.float32, device=dev) if t is not None and flag else None
-        dA, dD, dbias, dh0 = f32(A, True), f32(D, need[5]), f32(bias, need[7]), f32(h0, need[8])
-        scratch = torch.empty(s.workspaces()[2], dtype=torch.uint8, device=dev)
-        packed = s.pack(saved=saved, scratch=scratch, dout=dout, dhT=dhT, du=du, ddelta=ddelta, dz=dz, dB=dB, dC=dC,
-                        dA=dA, dD=dD, dbias=dbias, dh0=dh0)
-        _run("selective_scan backward", _lib.lib().atlas_sscan_backward, dev, packed)
-        return du, ddelta, dA, dB, dC, dD, dz, dbias, dh0, None, None, None, None
-
-
-def _no_steps(u: Tensor, N: int, h0: Tensor | None):
-    """Nothing to walk (no rows or no steps): the state passes through."""
-    hT = u.new_zeros(u.shape[0], u.shape[2], N, dtype=torch.float32) if h0 is None else h0.clone()
-    return torch.empty_like(u, memory_format=torch.contiguous_format), hT
-
-
-def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Tensor | None = None,
-                   z: Tensor | None = None, *, delta_bias: Tensor | None = None, delta_softplus: bool = False,
-                   initial_state: Tensor | None = None, lengths: Tensor | None = None, chunk: int = 0):
-    """Selective state space scan over [batch, steps, channels].
-
-    Per batch row, channel d (of group g) and state n:
-
-        dt_t = softplus(delta_t + delta_bias)   (delta_softplus False: delta_t + delta_bias)
-        h_t  = exp(dt_t A[d, n]) h_{t-1} + dt_t u_t B_t[g, n],   h_0 = initial_state (or 0)
-        out_t = (sum_n C_t[g, n] h_t + D u_t) silu(z_t)          (D, z None: left out)
-
-    u, delta, z [b, t, d] and B, C [b, t, n] or [b, t, g, n] (d a multiple of g, n up to 64) are all float32 or all
-    bfloat16, of any batch and step strides (halves of one projection are taken as they are); A [d, n],
-    D, delta_bias [d] and initial_state [b, d, n] are computed in float32, as is the state (an A of -inf as the lowest finite
-    value, so that a step with dt = 0 leaves the state). lengths [b] (int32 or
-    int64): steps at or past a row's length are not read, leave its state alone and give 0.
-    Returns (out [b, t, d] in u's type, final state [b, d, n] float32); both carry gradients to every
-    floating input. The sums over steps, states and channels are in float32 and in a fixed order, so the same call gives the
-    same bits. A training call keeps the states of every 8th step for its backward (d n / 8 floats a step).
-    One step without gradients runs one small kernel. chunk: steps per piece of a cut time axis (a multiple
-    of 32; 0 lets the library choose)."""
+def _scan_operands(u, delta, A, B, C, D, z, bias, h0, lengths, softplus, chunk) -> _Scan:
+    """The arguments of selective_scan, checked and laid out."""
     what = "selective_scan"
     if u.dim() != 3 or B.dim() not in (3, 4) or C.dim() != B.dim():
         raise ValueError(f"atlas_rnn_b200.{what}: expected u [b, t, d] and B, C [b, t, n] or [b, t, g, n], got "
@@ -243,26 +183,113 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D:
     if z is not None:
         _check(what, "z", z, (b, t, d), u.dtype, dev)
     A = _f32(what, "A", A, (d, n), dev)
-    D, bias = _f32(what, "D", D, (d,), dev), _f32(what, "delta_bias", delta_bias, (d,), dev)
-    h0 = _f32(what, "initial_state", initial_state, (b, d, n), dev)
+    D, bias = _f32(what, "D", D, (d,), dev), _f32(what, "delta_bias", bias, (d,), dev)
+    h0 = _f32(what, "initial_state", h0, (b, d, n), dev)
     lengths = _lengths(what, lengths, b, dev)
     _need_cuda(u, what)
-    if u.numel() == 0:
-        return _no_steps(u, n, h0)
-    u, delta, B, C = _rows(u), _rows(delta), _rows(B), _rows(C)
-    z = None if z is None else _rows(z)
-    keep = _wants_grad(u, delta, A, B, C, D, z, bias, h0)
-    if _through_autograd(keep):
-        return SelectiveScanFn.apply(u, delta, A, B, C, D, z, bias, h0, lengths, bool(delta_softplus), chunk, keep)
-    out, hT, _ = _Scan(u, delta, A, B, C, D, z, bias, h0, lengths, bool(delta_softplus), chunk).forward(keep=False)
-    return out, hT
+    return _Scan(_rows(u), _rows(delta), A, _rows(B), _rows(C), D, None if z is None else _rows(z), bias, h0, lengths,
+                 bool(softplus), chunk)
+
+
+class SelectiveScanFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, u, delta, A, B, C, D, z, bias, h0, lengths, softplus, chunk):
+        ctx.set_materialize_grads(False)
+        s = _scan_operands(u, delta, A, B, C, D, z, bias, h0, lengths, softplus, chunk)
+        out, hT, saved = s.forward(keep=any(ctx.needs_input_grad))
+        ctx.save_for_backward(s.u, s.delta, s.A, s.B, s.C, s.D, s.z, s.bias, s.h0, s.lengths, saved)
+        ctx.softplus, ctx.chunk, ctx.shapes = s.softplus, chunk, (B.shape, C.shape)
+        return out, hT
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dhT):
+        u, delta, A, B, C, D, z, bias, h0, lengths, saved = ctx.saved_tensors
+        need = ctx.needs_input_grad  # (u, delta, A, B, C, D, z, bias, h0, ...)
+        s = _Scan(u, delta, A, B, C, D, z, bias, h0, lengths, ctx.softplus, ctx.chunk)
+        dev = u.device
+        if u.numel() == 0:  # the state passed through
+            zeros = [None if t is None else torch.zeros_like(t) for t in (u, delta, A, B, C, D, z, bias, h0)]
+            zeros[3], zeros[4] = zeros[3].view(ctx.shapes[0]), zeros[4].view(ctx.shapes[1])
+            return *zeros[:8], zeros[8] if dhT is None else dhT, None, None, None
+        dout = torch.zeros(u.shape, dtype=u.dtype, device=dev) if dout is None else _rows(dout)
+        dhT = None if dhT is None else dhT.contiguous()
+        rows = lambda: torch.empty(u.shape, dtype=u.dtype, device=dev)
+        du, ddelta, dz = rows(), rows(), rows() if z is not None else None
+        dB = torch.empty(B.shape, dtype=u.dtype, device=dev) if need[3] or need[4] else None
+        dC = torch.empty(C.shape, dtype=u.dtype, device=dev) if need[3] or need[4] else None
+        f32 = lambda t, flag: torch.empty(t.shape, dtype=torch.float32, device=dev) if t is not None and flag else None
+        dA, dD, dbias, dh0 = f32(A, True), f32(D, need[5]), f32(bias, need[7]), f32(h0, need[8])
+        scratch = torch.empty(s.workspaces()[2], dtype=torch.uint8, device=dev)
+        packed = s.pack(saved=saved, scratch=scratch, dout=dout, dhT=dhT, du=du, ddelta=ddelta, dz=dz, dB=dB, dC=dC,
+                        dA=dA, dD=dD, dbias=dbias, dh0=dh0)
+        _run("selective_scan backward", _lib.lib().atlas_sscan_backward, dev, packed)
+        if dB is not None:
+            dB, dC = dB.view(ctx.shapes[0]), dC.view(ctx.shapes[1])
+        return du, ddelta, dA, dB, dC, dD, dz, dbias, dh0, None, None, None
+
+
+def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Tensor | None = None,
+                   z: Tensor | None = None, *, delta_bias: Tensor | None = None, delta_softplus: bool = False,
+                   initial_state: Tensor | None = None, lengths: Tensor | None = None, chunk: int = 0):
+    """Selective state space scan over [batch, steps, channels].
+
+    Per batch row, channel d (of group g) and state n:
+
+        dt_t = softplus(delta_t + delta_bias)   (delta_softplus False: delta_t + delta_bias)
+        h_t  = exp(dt_t A[d, n]) h_{t-1} + dt_t u_t B_t[g, n],   h_0 = initial_state (or 0)
+        out_t = (sum_n C_t[g, n] h_t + D u_t) silu(z_t)          (D, z None: left out)
+
+    u, delta, z [b, t, d] and B, C [b, t, n] or [b, t, g, n] (d a multiple of g, n up to 64) are all float32 or all
+    bfloat16, of any batch and step strides (halves of one projection are taken as they are); A [d, n],
+    D, delta_bias [d] and initial_state [b, d, n] are computed in float32, as is the state (an A of -inf as the lowest finite
+    value, so that a step with dt = 0 leaves the state). lengths [b] (int32 or
+    int64): steps at or past a row's length are not read, leave its state alone and give 0.
+    Returns (out [b, t, d] in u's type, final state [b, d, n] float32); both carry gradients to every
+    floating input. The sums over steps, states and channels are in float32 and in a fixed order, so the same call gives the
+    same bits. A training call keeps the states of every 8th step for its backward (d n / 8 floats a step).
+    One step without gradients runs one small kernel. chunk: steps per piece of a cut time axis (a multiple
+    of 32; 0 lets the library choose)."""
+    if _through_autograd(u, delta, A, B, C, D, z, delta_bias, initial_state):
+        return SelectiveScanFn.apply(u, delta, A, B, C, D, z, delta_bias, initial_state, lengths, delta_softplus, chunk)
+    return _scan_operands(u, delta, A, B, C, D, z, delta_bias, initial_state, lengths, delta_softplus,
+                          chunk).forward(keep=False)[:2]
 
 
 # ---- causal convolution ----------------------------------------------------------------------
 
+def _conv_operands(x, weight, bias, init, lengths, activation):
+    """The arguments of causal_conv1d, checked and laid out."""
+    what = "causal_conv1d"
+    if x.dim() != 3:
+        raise ValueError(f"atlas_rnn_b200.{what}: expected x [b, t, c], got {tuple(x.shape)}")
+    if x.dtype not in _IO:
+        raise TypeError(f"atlas_rnn_b200.{what}: x must be float32 or bfloat16, not {x.dtype}")
+    if activation not in (None, "silu"):
+        raise ValueError(f"atlas_rnn_b200.{what}: activation must be None or 'silu', not {activation!r}")
+    B, T, C = x.shape
+    _check_sizes(what, B, T, C, MAX_CONV_CHANNELS)
+    K = weight.shape[-1]
+    if not 2 <= K <= MAX_CONV_K:
+        raise ValueError(f"atlas_rnn_b200.{what}: 2 to {MAX_CONV_K} taps, not {K}")
+    dev = x.device
+    w = _f32(what, "weight", weight, (C, 1, K) if weight.dim() == 3 else (C, K), dev)
+    bias = _f32(what, "bias", bias, (C,), dev)
+    if init is not None:
+        _check(what, "initial_state", init, (B, K - 1, C), x.dtype, dev)
+        if not init.is_contiguous():
+            init = init.contiguous()
+    lengths = _lengths(what, lengths, B, dev)
+    _need_cuda(x, what)
+    return _rows(x), w, bias, init, lengths, int(activation == "silu")
+
+
 def _conv_forward(x, w, bias, init, lengths, silu):
     B, T, C = x.shape
     K = w.shape[-1]
+    if x.numel() == 0:
+        final = x.new_zeros(B, K - 1, C) if init is None else init.clone()
+        return torch.empty_like(x, memory_format=torch.contiguous_format), final
     y = torch.empty(B, T, C, dtype=x.dtype, device=x.device)
     final = torch.empty(B, K - 1, C, dtype=x.dtype, device=x.device)
     _run("causal_conv1d forward", _lib.lib().atlas_causal_conv_forward, x.device, x.data_ptr(), x.stride(0),
@@ -273,11 +300,11 @@ def _conv_forward(x, w, bias, init, lengths, silu):
 
 class CausalConv1dFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, init, lengths, silu):
+    def forward(ctx, x, w, bias, init, lengths, activation):
         ctx.set_materialize_grads(False)
-        y, final = _conv_forward(x, w, bias, init, lengths, silu)
-        ctx.save_for_backward(x, w, bias, init, lengths)
-        ctx.silu = silu
+        *tensors, ctx.silu = _conv_operands(x, w, bias, init, lengths, activation)
+        y, final = _conv_forward(*tensors, ctx.silu)
+        ctx.save_for_backward(*tensors)
         return y, final
 
     @staticmethod
@@ -287,6 +314,9 @@ class CausalConv1dFn(torch.autograd.Function):
         B, T, C = x.shape
         K = w.shape[-1]
         dev = x.device
+        if x.numel() == 0:  # the state passed through
+            dx, dw, dbias, d_init = (None if t is None else torch.zeros_like(t) for t in (x, w, bias, init))
+            return dx, dw, dbias, d_init if d_final is None or init is None else d_final, None, None
         dy = torch.zeros(B, T, C, dtype=x.dtype, device=dev) if dy is None else _rows(dy)
         d_final = None if d_final is None else d_final.contiguous()
         dx = torch.empty(B, T, C, dtype=x.dtype, device=dev)
@@ -313,32 +343,6 @@ def causal_conv1d(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, acti
     before the first step (None: zeros). lengths [b]: steps at or past a row's length are not read and give 0.
     Returns (y, final state [b, K - 1, c]: the last K - 1 inputs of each row, the next call's
     initial_state), both with gradients to x, weight, bias and initial_state."""
-    what = "causal_conv1d"
-    if x.dim() != 3:
-        raise ValueError(f"atlas_rnn_b200.{what}: expected x [b, t, c], got {tuple(x.shape)}")
-    if x.dtype not in _IO:
-        raise TypeError(f"atlas_rnn_b200.{what}: x must be float32 or bfloat16, not {x.dtype}")
-    if activation not in (None, "silu"):
-        raise ValueError(f"atlas_rnn_b200.{what}: activation must be None or 'silu', not {activation!r}")
-    B, T, C = x.shape
-    _check_sizes(what, B, T, C, MAX_CONV_CHANNELS)
-    K = weight.shape[-1]
-    if not 2 <= K <= MAX_CONV_K:
-        raise ValueError(f"atlas_rnn_b200.{what}: 2 to {MAX_CONV_K} taps, not {K}")
-    dev = x.device
-    w = _f32(what, "weight", weight, (C, 1, K) if weight.dim() == 3 else (C, K), dev)
-    bias = _f32(what, "bias", bias, (C,), dev)
-    if initial_state is not None:
-        _check(what, "initial_state", initial_state, (B, K - 1, C), x.dtype, dev)
-        if not initial_state.is_contiguous():
-            initial_state = initial_state.contiguous()
-    lengths = _lengths(what, lengths, B, dev)
-    _need_cuda(x, what)
-    silu = int(activation == "silu")
-    if x.numel() == 0:
-        final = x.new_zeros(B, K - 1, C) if initial_state is None else initial_state.clone()
-        return torch.empty_like(x, memory_format=torch.contiguous_format), final
-    x = _rows(x)
-    if _through_autograd(_wants_grad(x, w, bias, initial_state)):
-        return CausalConv1dFn.apply(x, w, bias, initial_state, lengths, silu)
-    return _conv_forward(x, w, bias, initial_state, lengths, silu)
+    if _through_autograd(x, weight, bias, initial_state):
+        return CausalConv1dFn.apply(x, weight, bias, initial_state, lengths, activation)
+    return _conv_forward(*_conv_operands(x, weight, bias, initial_state, lengths, activation))

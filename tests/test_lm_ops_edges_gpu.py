@@ -1,0 +1,28 @@
+"""GPU: calls of the language-model operators at the edges of what their documentation allows."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("b,t", [(0, 5), (2, 0)])
+def test_calls_without_steps_carry_gradients(native_lib, b, t):
+    """No rows or no steps: every input gets a gradient, of zeros but for what passes the state through."""
+    from atlas_rnn_b200 import causal_conv1d, selective_scan
+    leaf = lambda *s: torch.randn(*s, device="cuda").requires_grad_()
+    x = dict(u=leaf(b, t, 6), delta=leaf(b, t, 6), A=leaf(6, 4), B=leaf(b, t, 4), C=leaf(b, t, 4), D=leaf(6), z=leaf(b, t, 6),
+             delta_bias=leaf(6), initial_state=leaf(b, 6, 4))
+    out, hT = selective_scan(**x)
+    assert out.shape == (b, t, 6) and torch.equal(hT, x["initial_state"])
+    (out.sum() + 3 * hT.sum()).backward()
+    for k, v in x.items():
+        assert torch.equal(v.grad, torch.full_like(v, 3.0 if k == "initial_state" else 0.0)), k
+    c = dict(x=leaf(b, t, 6), weight=leaf(6, 1, 4), bias=leaf(6), initial_state=leaf(b, 3, 6))
+    y, final = causal_conv1d(**c)
+    assert y.shape == (b, t, 6) and torch.equal(final, c["initial_state"])
+    (y.sum() + 3 * final.sum()).backward()
+    for k, v in c.items():
+        assert torch.equal(v.grad, torch.full_like(v, 3.0 if k == "initial_state" else 0.0)), k
+    u = leaf(b, t, 6)
+    causal_conv1d(u, c["weight"])[0].sum().backward()  # the outputs alone, without a state
+    assert torch.equal(u.grad, torch.zeros_like(u))
