@@ -38,20 +38,7 @@ def _setting(name: str, value, lead: tuple, device, dtype, lowest, highest):
     return 0, value.to(dtype).contiguous()
 
 
-def sample_tokens(logits: Tensor, noise: Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> Tensor:
-    """One token per row of ``logits`` [..., V] (float32 or bfloat16), drawn with the uniforms ``noise`` [..., V]
-    (float32 in [0, 1)). In the order of descending logit, ties by lowest index, the filters are, on softmax(logits):
-
-        top_k   the first top_k tokens (0: all)
-        top_p   of those, the ones with less than top_p of their probability before them, the first always (1: all)
-        min_p   of those, the ones with at least min_p times the first one's probability
-
-    and the token is the kept one with the largest logits / temperature - log(-log(noise)); temperature 0 (or below
-    1e-30) gives the first token. The filters see the logits without the temperature, as ``min_p_filter`` before ``gumbel_sample`` does: divide
-    the logits beforehand for filters on the tempered distribution. Each setting is a number or a tensor with one value
-    per row. Masked tokens are -inf (NaN counts as -inf); a row with nothing above -inf gives 0.
-    V up to 2^24 - 16. Returns int64 [...], the same whatever the batch: scores are compared in float64, the probabilities
-    that the filters add up are exact to 2^-23 each."""
+def _sample(logits, noise, temperature, top_k, top_p, min_p) -> Tensor:
     what = "sample_tokens"
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"atlas_rnn_b200.{what}: expected logits [..., V], got {tuple(logits.shape)}")
@@ -76,3 +63,35 @@ def sample_tokens(logits: Tensor, noise: Tensor, *, temperature=1.0, top_k=0, to
          _SAMPLE.pack(x.data_ptr(), u.data_ptr(), out.data_ptr(), x.shape[0], V, x.stride(0), u.stride(0), t, p, m,
                       min(k, 0x7fffffff), _ptr(t_row), _ptr(p_row), _ptr(m_row), _ptr(k_row), _IO[x.dtype]))
     return out
+
+
+class SampleTokensFn(torch.autograd.Function):
+    """``sample_tokens`` for torch.jit.trace, which sees no calls of the library outside such a function."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        out = _sample(*args)
+        ctx.mark_non_differentiable(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, _):
+        return (None,) * 6
+
+
+def sample_tokens(logits: Tensor, noise: Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> Tensor:
+    """One token per row of ``logits`` [..., V] (float32 or bfloat16), drawn with the uniforms ``noise`` [..., V]
+    (float32 in [0, 1)). In the order of descending logit, ties by lowest index, the filters are, on softmax(logits):
+
+        top_k   the first top_k tokens (0: all)
+        top_p   of those, the ones with less than top_p of their probability before them, the first always (1: all)
+        min_p   of those, the ones with at least min_p times the first one's probability
+
+    and the token is the kept one with the largest logits / temperature - log(-log(noise)); temperature 0 (or below
+    1e-30) gives the first token. The filters see the logits without the temperature, as ``min_p_filter`` before ``gumbel_sample`` does: divide
+    the logits beforehand for filters on the tempered distribution. Each setting is a number or a tensor with one value
+    per row. Masked tokens are -inf (NaN counts as -inf); a row with nothing above -inf gives 0.
+    V up to 2^24 - 16. Returns int64 [...], the same whatever the batch: scores are compared in float64, the probabilities
+    that the filters add up are exact to 2^-23 each."""
+    call = SampleTokensFn.apply if torch.jit.is_tracing() else _sample
+    return call(logits, noise, temperature, top_k, top_p, min_p)

@@ -83,9 +83,12 @@ def _lengths(what: str, lengths, batch: int, device) -> Tensor | None:
 
 
 def _through_autograd(*tensors) -> bool:
-    """Whether a call goes through its autograd function: for a backward pass, and with a forward-mode tangent, which the
-    function refuses (a call past it would drop the tangent). Else the call itself saves the detour's time."""
-    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or _has_tangent(*tensors)
+    """Whether a call goes through its autograd function: for a backward pass; with a forward-mode tangent, which the
+    function refuses (a call past it would drop the tangent); and for a trace, which would have no more of a call past it than
+    the allocation of the outputs. Else the call itself saves the detour's time. The function holds the checks and layouts
+    too: a traced call does them on the inputs that it is run with."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) \
+        or torch.jit.is_tracing() or _has_tangent(*tensors)
 
 
 def _run(what: str, fn, device, *args):
@@ -137,7 +140,8 @@ class _Scan:
 
     def workspaces(self):
         u = self.u
-        return _scan_workspaces(u.device.index, *u.shape, self.B.shape[3], self.B.shape[2], _IO[u.dtype], self.chunk)
+        sizes = map(int, (*u.shape, self.B.shape[3], self.B.shape[2]))  # while a trace is taken they are tensors
+        return _scan_workspaces(u.device.index, *sizes, _IO[u.dtype], self.chunk)
 
     def forward(self, keep: bool):
         """(out, final state, kept states or None)."""

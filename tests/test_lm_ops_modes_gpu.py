@@ -1,5 +1,8 @@
 """GPU: the language-model operators under torch's other ways of calling a function: forward-mode differentiation is
-refused, as by the package's other operators."""
+refused, as by the package's other operators; torch.jit.trace has the call in it, so a traced call gives the same bits, checks
+its inputs, and takes other sizes and strides than the traced ones."""
+import warnings
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -55,3 +58,71 @@ def test_dual_level_keeps_the_bits(native_lib, t):
     with forward_ad.dual_level():
         got = *selective_scan(**x, delta_softplus=True), *causal_conv1d(x["u"], x["A"])
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def traced(f, *example):
+    with torch.no_grad(), warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        return torch.jit.trace(f, example)
+
+
+def same(f, module, *args):
+    got, want = module(*args), f(*args)
+    got, want = (got, want) if isinstance(got, tuple) else ((got,), (want,))
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and len(got) == len(want)
+
+
+@pytest.mark.parametrize("t", [1, 40])
+def test_traced_scan(native_lib, t):
+    from atlas_rnn_b200 import selective_scan
+    names = ("u", "delta", "A", "B", "C", "z", "initial_state")
+    f = lambda *a: selective_scan(**dict(zip(names, a)), delta_softplus=True)
+    args = lambda *s, seed: [scan_inputs(*s, seed=seed)[k] for k in names]
+    m = traced(f, *args(2, t, 6, 4, seed=1))
+    same(f, m, *args(2, t, 6, 4, seed=10))
+    other = args(3, t + 2, 10, 5, seed=20)
+    same(f, m, *other)
+    other[0] = other[0].transpose(1, 2).contiguous().transpose(1, 2)  # channels far apart
+    other[2] = other[2].double()
+    same(f, m, *other)
+    leaves = [[v.detach().clone().requires_grad_() for v in other] for _ in range(2)]
+    for out, hT in (f(*leaves[0]), m(*leaves[1])):
+        (out.sum() + hT.sum()).backward()
+    assert all(torch.equal(a.grad, b.grad) for a, b in zip(*leaves))
+    with pytest.raises(Exception, match="delta must have shape"):
+        m(other[0], other[1][:, :-1], *other[2:])
+
+
+@pytest.mark.parametrize("t", [1, 40])
+def test_traced_convolution(native_lib, t):
+    from atlas_rnn_b200 import causal_conv1d
+    f = lambda x, w, b, s: causal_conv1d(x, w, b, initial_state=s, activation="silu")
+    args = lambda b, t, c, seed: [rand(b, t, c, seed=seed), rand(c, 1, 4, seed=seed + 1), rand(c, seed=seed + 2),
+                                  rand(b, 3, c, seed=seed + 3)]
+    m = traced(f, *args(2, t, 6, seed=1))
+    same(f, m, *args(2, t, 6, seed=10))
+    other = args(3, t + 2, 9, seed=20)
+    same(f, m, *other)
+    other[0] = other[0].transpose(1, 2).contiguous().transpose(1, 2)
+    other[1] = other[1].to(torch.bfloat16)
+    same(f, m, *other)
+    leaves = [[v.detach().clone().requires_grad_() for v in other] for _ in range(2)]
+    for y, final in (f(*leaves[0]), m(*leaves[1])):
+        (y.sum() + final.sum()).backward()
+    assert all(torch.equal(a.grad, b.grad) for a, b in zip(*leaves))
+    with pytest.raises(Exception, match="initial_state must have shape"):
+        m(*other[:3], other[3][:, :-1])
+
+
+def test_traced_sampling(native_lib):
+    from atlas_rnn_b200 import sample_tokens
+    f = lambda l, u, k: sample_tokens(l, u, temperature=0.8, top_p=0.9, top_k=k)
+    args = lambda rows, V, seed: [rand(rows, V, seed=seed), rand(rows, V, seed=seed + 1).sigmoid(),
+                                  torch.arange(1, rows + 1, device="cuda")]
+    m = traced(f, *args(3, 50, seed=1))
+    same(f, m, *args(3, 50, seed=10))
+    l, u, k = args(5, 700, seed=20)
+    same(f, m, l, u, k)
+    same(f, m, l.t().contiguous().t(), u, k)
+    with pytest.raises(Exception, match="noise must have shape"):
+        m(l, u[:, :-1], k)
