@@ -289,8 +289,9 @@ def memory_recurrence(k: Tensor, q: Tensor, v: Tensor, lr: Tensor, decay: Tensor
     Returns (y [N,T,d_v], S_end (clamped to +-100), Z_end or None, new omega buffer or None).
     io tensors run in bfloat16 when k is bfloat16 or bf16 autocast is on (as autocast runs the
     reference's einsums), else float32; states in float32.
-    A single token (T = 1) with no autograd graph to record and no forward-mode tangent
-    (which the autograd function refuses) runs as one decode
+    A single token (T = 1) with no autograd graph to record, no forward-mode tangent
+    (which the autograd function refuses) and outside torch.jit.trace (which would see
+    the outputs' allocation alone) runs as one decode
     kernel (atlas_mem_decode_step) unless the tensor feature map is on.
     ref_mode 'call' (default, the reference's semantics): every token's delta uses S_ref.
     ref_mode 'chunk': the chunk-start state is the reference state -- the sequence runs as
@@ -342,7 +343,7 @@ def memory_recurrence(k: Tensor, q: Tensor, v: Tensor, lr: Tensor, decay: Tensor
     args = (_io(k, io), _io(q, io), _io(v, io), _io(lr, io), _io(decay, io), _io(beta, io), _io(gate, io),
             f32(S_ref), f32(S0), Z0c, buf, projc)
     inputs = (k, q, v, lr, decay, beta, gate, S_ref, S0, Z0, omega_buffer)
-    needs_grad = _has_tangent(*inputs) or torch.is_grad_enabled() and any(
+    needs_grad = torch.jit.is_tracing() or _has_tangent(*inputs) or torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in inputs)
     if (heads_padded_from is None and k.shape[1] == 1 and not needs_grad
             and decode_supported(spec, k.shape[-1], S_ref.shape[-1], v.shape[-1])):

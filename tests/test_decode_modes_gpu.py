@@ -1,10 +1,14 @@
-"""GPU: memory_recurrence of one token under forward-mode differentiation: refused, as for longer calls."""
+"""GPU: memory_recurrence of one token under forward-mode differentiation (refused, as for longer calls) and
+torch.jit.trace (the call's results, by the kernels of longer calls: within fp32 rounding of the decode kernel's)."""
+import warnings
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
 from atlas_rnn_b200 import memory_recurrence
 from atlas_rnn_b200.workloads import Workload, make_inputs
+from tests.helpers import TOL_F32, rel_l2
 
 pytestmark = pytest.mark.gpu
 NAMES = ("k", "q", "v", "lr", "decay", "beta", "S0", "Z0")
@@ -29,3 +33,11 @@ def test_forward_mode_of_one_token_is_refused(native_lib, name):
         x[at] = forward_ad.make_dual(x[at], torch.ones_like(x[at]))
         with pytest.raises(NotImplementedError):
             call(*x)
+
+
+def test_traced_one_token(native_lib):
+    with torch.no_grad(), warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        m = torch.jit.trace(call, tuple(inputs(1)))
+    for got, want in zip(m(*inputs(2)), call(*inputs(2))):
+        assert rel_l2(got, want) <= TOL_F32
