@@ -21,35 +21,66 @@ MAX_ENTRIES = 1024  # teacher entries per row
 _DISTILL = struct.Struct("@8P4qfi")
 
 
+def _operands(logits, teacher_values, teacher_indices, temperature):
+    """The arguments of distill_loss, checked and laid out: rows of logits, of values and of indices. Part of the autograd
+    function, so that a traced call checks the inputs that it is run with."""
+    what = "distill_loss"
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"atlas_rnn_b200.{what}: expected logits [..., V], got {tuple(logits.shape)}")
+    if logits.dtype not in _IO:
+        raise TypeError(f"atlas_rnn_b200.{what}: logits must be float32 or bfloat16, not {logits.dtype}")
+    if teacher_values.dim() < 1 or not 1 <= teacher_values.shape[-1] <= MAX_ENTRIES:
+        raise ValueError(f"atlas_rnn_b200.{what}: expected teacher_values [..., K] with K from 1 to {MAX_ENTRIES}, got "
+                         f"{tuple(teacher_values.shape)}")
+    if not teacher_values.is_floating_point():
+        raise TypeError(f"atlas_rnn_b200.{what}: teacher_values must be a floating type, not {teacher_values.dtype}")
+    if teacher_indices.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"atlas_rnn_b200.{what}: teacher_indices must be int32 or int64, not {teacher_indices.dtype}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"atlas_rnn_b200.{what}: temperature must be from 1e-6 to 1e6, not {temperature}")
+    lead, V, K = logits.shape[:-1], logits.shape[-1], teacher_values.shape[-1]
+    if V > 0x7ffffff0:
+        raise ValueError(f"atlas_rnn_b200.{what}: {V} tokens are too many")
+    _check(what, "teacher_values", teacher_values, (*lead, K), None, logits.device)
+    _check(what, "teacher_indices", teacher_indices, (*lead, K), None, logits.device)
+    _need_cuda(logits, what)
+    x = logits.reshape(-1, V)
+    x = x if x.stride(1) == 1 or V == 1 else x.contiguous()
+    return (x, teacher_values.to(torch.float32).reshape(-1, K).contiguous(),
+            teacher_indices.to(torch.int64).reshape(-1, K).contiguous())
+
+
 class DistillLossFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, values, indices, temperature):
-        rows, V = logits.shape
-        dev = logits.device
-        loss = torch.empty(rows, dtype=torch.float32, device=dev)
-        valid = torch.empty(rows, dtype=torch.float32, device=dev)
+    def forward(ctx, logits, teacher_values, teacher_indices, temperature):
+        x, values, indices = _operands(logits, teacher_values, teacher_indices, temperature)
+        rows, V = x.shape
+        dev = x.device
+        loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
+        valid = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
         stats = torch.empty(rows, 4, dtype=torch.float32, device=dev)
-        _run("distill_loss forward", _lib.lib().atlas_distill_forward, dev,
-             _DISTILL.pack(logits.data_ptr(), values.data_ptr(), indices.data_ptr(), loss.data_ptr(), valid.data_ptr(),
-                           stats.data_ptr(), 0, 0, rows, V, values.shape[1], logits.stride(0), temperature,
-                           _IO[logits.dtype]))
-        ctx.save_for_backward(logits, values, indices, stats)
-        ctx.temperature = temperature
+        if rows:
+            _run("distill_loss forward", _lib.lib().atlas_distill_forward, dev,
+                 _DISTILL.pack(x.data_ptr(), values.data_ptr(), indices.data_ptr(), loss.data_ptr(), valid.data_ptr(),
+                               stats.data_ptr(), 0, 0, rows, V, values.shape[1], x.stride(0), temperature, _IO[x.dtype]))
+        ctx.save_for_backward(x, values, indices, stats)
+        ctx.temperature, ctx.shape = temperature, logits.shape
         ctx.mark_non_differentiable(valid)
         return loss, valid
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss, _):
-        logits, values, indices, stats = ctx.saved_tensors
-        rows, V = logits.shape
-        dev = logits.device
-        dlogits = torch.empty(rows, V, dtype=logits.dtype, device=dev)
+        x, values, indices, stats = ctx.saved_tensors
+        rows, V = x.shape
+        dev = x.device
+        dlogits = torch.empty(ctx.shape, dtype=x.dtype, device=dev)
         dloss = dloss.contiguous()
-        _run("distill_loss backward", _lib.lib().atlas_distill_backward, dev,
-             _DISTILL.pack(logits.data_ptr(), values.data_ptr(), indices.data_ptr(), 0, 0, stats.data_ptr(),
-                           dloss.data_ptr(), dlogits.data_ptr(), rows, V, values.shape[1], logits.stride(0),
-                           ctx.temperature, _IO[logits.dtype]))
+        if rows:
+            _run("distill_loss backward", _lib.lib().atlas_distill_backward, dev,
+                 _DISTILL.pack(x.data_ptr(), values.data_ptr(), indices.data_ptr(), 0, 0, stats.data_ptr(),
+                               dloss.data_ptr(), dlogits.data_ptr(), rows, V, values.shape[1], x.stride(0),
+                               ctx.temperature, _IO[x.dtype]))
         return dlogits, None, None, None
 
 
@@ -67,36 +98,9 @@ def distill_loss(logits: Tensor, teacher_values: Tensor, teacher_indices: Tensor
 
     and 0 (without a gradient) for a row that has no entries. reduction 'none' returns float32 [...]; 'sum' the sum; 'mean'
     the mean over the rows with entries (0 when there are none). Gradients go to the logits alone."""
-    what = "distill_loss"
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"atlas_rnn_b200.{what}: expected logits [..., V], got {tuple(logits.shape)}")
-    if logits.dtype not in _IO:
-        raise TypeError(f"atlas_rnn_b200.{what}: logits must be float32 or bfloat16, not {logits.dtype}")
-    if teacher_values.dim() < 1 or not 1 <= teacher_values.shape[-1] <= MAX_ENTRIES:
-        raise ValueError(f"atlas_rnn_b200.{what}: expected teacher_values [..., K] with K from 1 to {MAX_ENTRIES}, got "
-                         f"{tuple(teacher_values.shape)}")
-    if not teacher_values.is_floating_point():
-        raise TypeError(f"atlas_rnn_b200.{what}: teacher_values must be a floating type, not {teacher_values.dtype}")
-    if teacher_indices.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"atlas_rnn_b200.{what}: teacher_indices must be int32 or int64, not {teacher_indices.dtype}")
     if reduction not in ("none", "mean", "sum"):
-        raise ValueError(f"atlas_rnn_b200.{what}: reduction must be 'none', 'mean' or 'sum', not {reduction!r}")
-    if not 1e-6 <= temperature <= 1e6:
-        raise ValueError(f"atlas_rnn_b200.{what}: temperature must be from 1e-6 to 1e6, not {temperature}")
-    lead, V, K = logits.shape[:-1], logits.shape[-1], teacher_values.shape[-1]
-    if V > 0x7ffffff0:
-        raise ValueError(f"atlas_rnn_b200.{what}: {V} tokens are too many")
-    _check(what, "teacher_values", teacher_values, (*lead, K), None, logits.device)
-    _check(what, "teacher_indices", teacher_indices, (*lead, K), None, logits.device)
-    _need_cuda(logits, what)
-    if logits.numel() == 0:
-        rows = logits.float().sum(-1)  # no rows
-        return rows if reduction == "none" else rows.sum()
-    x = logits.reshape(-1, V)
-    x = x if x.stride(1) == 1 or V == 1 else x.contiguous()
-    values = teacher_values.detach().to(torch.float32).reshape(-1, K).contiguous()
-    indices = teacher_indices.to(torch.int64).reshape(-1, K).contiguous()
-    loss, valid = DistillLossFn.apply(x, values, indices, float(temperature))
+        raise ValueError(f"atlas_rnn_b200.distill_loss: reduction must be 'none', 'mean' or 'sum', not {reduction!r}")
+    loss, valid = DistillLossFn.apply(logits, teacher_values.detach(), teacher_indices, float(temperature))
     if reduction == "none":
-        return loss.reshape(lead)
+        return loss
     return loss.sum() if reduction == "sum" else loss.sum() / valid.sum().clamp(min=1.0)

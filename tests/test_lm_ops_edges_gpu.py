@@ -26,3 +26,15 @@ def test_calls_without_steps_carry_gradients(native_lib, b, t):
     u = leaf(b, t, 6)
     causal_conv1d(u, c["weight"])[0].sum().backward()  # the outputs alone, without a state
     assert torch.equal(u.grad, torch.zeros_like(u))
+
+
+@pytest.mark.parametrize("lead", [(0,), (2, 0), (0, 3)])
+def test_distillation_of_no_rows(native_lib, lead):
+    from atlas_rnn_b200 import distill_loss
+    for reduction, shape in (("none", lead), ("sum", ()), ("mean", ())):
+        x = torch.zeros(*lead, 50, device="cuda", requires_grad=True)
+        loss = distill_loss(x, torch.zeros(*lead, 4, device="cuda", requires_grad=True),
+                            torch.zeros(*lead, 4, dtype=torch.int64, device="cuda"), reduction=reduction)
+        assert loss.shape == shape and loss.sum() == 0
+        loss.sum().backward()
+        assert x.grad.shape == x.shape

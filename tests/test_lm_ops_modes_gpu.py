@@ -126,3 +126,20 @@ def test_traced_sampling(native_lib):
     same(f, m, l.t().contiguous().t(), u, k)
     with pytest.raises(Exception, match="noise must have shape"):
         m(l, u[:, :-1], k)
+
+
+def test_traced_distillation(native_lib):
+    from atlas_rnn_b200 import distill_loss
+    f = lambda x, v, i: distill_loss(x, v, i, temperature=2.0)
+
+    def args(rows, V, K, seed):
+        g = torch.Generator().manual_seed(seed)
+        return [rand(rows, V, seed=seed), rand(rows, K, seed=seed + 1), torch.randint(0, V, (rows, K), generator=g).cuda()]
+
+    m = traced(f, *args(3, 50, 4, seed=1))
+    same(f, m, *args(3, 50, 4, seed=10))
+    x, v, i = args(5, 700, 6, seed=20)
+    same(f, m, x, v, i)
+    same(f, m, x.t().contiguous().t(), v.double(), i.int())
+    with pytest.raises(Exception, match="teacher_values must have shape"):
+        m(x, v[:3], i)
