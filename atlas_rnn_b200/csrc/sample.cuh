@@ -239,11 +239,12 @@ __global__ void __launch_bounds__(NT) k_sample(const SampleArgs a) {
   r.ring = reinterpret_cast<typename Row<IO, NT>::Ring*>(sm_raw + sizeof(Smem));
   const float* noise = a.noise + row * a.noise_stride;
 
-  const double temperature = fmin(a.temperature_row ? (double)a.temperature_row[row] : a.temperature, 1e300);
+  const double t_given = a.temperature_row ? (double)a.temperature_row[row] : a.temperature;
+  const double temperature = fmin(t_given, 1e300);  // a NaN becomes 1e300: it is caught before
   const double top_p = a.top_p_row ? (double)a.top_p_row[row] : a.top_p;
   const double min_p = a.min_p_row ? (double)a.min_p_row[row] : a.min_p;
   int64_t k = a.top_k_row ? a.top_k_row[row] : a.top_k;
-  if (!(top_p > 0.0) || !(min_p <= 1.0) || !(temperature >= 1e-30)) k = 1;  // nothing but the first token
+  if (!(top_p > 0.0) || !(min_p <= 1.0) || !(t_given >= 1e-30)) k = 1;  // nothing but the first token (NaNs too)
   const bool need_k = k >= 1 && k < a.V, need_p = top_p < 1.0;
   const float inv_t = (float)(1.0 / fmax(temperature, 1e-30));
 

@@ -90,7 +90,8 @@ def sample_tokens(logits: Tensor, noise: Tensor, *, temperature=1.0, top_k=0, to
     and the token is the kept one with the largest logits / temperature - log(-log(noise)); temperature 0 (or below
     1e-30) gives the first token. The filters see the logits without the temperature, as ``min_p_filter`` before ``gumbel_sample`` does: divide
     the logits beforehand for filters on the tempered distribution. Each setting is a number or a tensor with one value
-    per row. Masked tokens are -inf (NaN counts as -inf); a row with nothing above -inf gives 0.
+    per row (a row with a NaN among them gets its first token). Masked tokens are -inf (NaN counts as -inf); a row with
+    nothing above -inf gives 0.
     V up to 2^24 - 16. Returns int64 [...], the same whatever the batch: scores are compared in float64, the probabilities
     that the filters add up are exact to 2^-23 each."""
     call = SampleTokensFn.apply if torch.jit.is_tracing() else _sample

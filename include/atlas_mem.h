@@ -472,8 +472,8 @@ int atlas_causal_conv_backward(const void* x, int64_t x_sb, int64_t x_st, const 
  *   top-p: of those, the tokens with less than top_p of their mass exp(logit) before them (the first always; >= 1: all);
  *   min-p: of those, the tokens with at least min_p times the first one's probability (the first always);
  *   out = argmax over the kept of logit / temperature - log(-log u), u from noise [rows, V] fp32 in [0, 1], clamped as
- *   gumbel_noise clamps (1e-20); a temperature below 1e-30: the first token. A row without any logit above -inf gives 0.
- * V <= 2^24 - 16.
+ *   gumbel_noise clamps (1e-20); a temperature below 1e-30, or a NaN as temperature, top_p or min_p: the first token. A row
+ *   without any logit above -inf gives 0. V <= 2^24 - 16.
  * Each setting is one value, or an array of one per row where its _row pointer is given. */
 typedef struct AtlasSample {
   const void* logits;

@@ -38,3 +38,21 @@ def test_distillation_of_no_rows(native_lib, lead):
         assert loss.shape == shape and loss.sum() == 0
         loss.sum().backward()
         assert x.grad.shape == x.shape
+
+
+@pytest.mark.parametrize("rows,V", [(4, 300), (2, 40000)])
+def test_settings_per_row_that_are_nan_give_the_first_token(native_lib, rows, V):
+    """As a comparison with a NaN keeps nothing but the first token: in each of the three settings that have NaNs."""
+    from atlas_rnn_b200 import sample_tokens
+    g = torch.Generator().manual_seed(5)
+    l, u = torch.randn(rows, V, generator=g).cuda(), torch.rand(rows, V, generator=g).cuda()
+    want = sample_tokens(l, u)
+    bad = torch.full((rows,), float("nan"), device="cuda")
+    bad[1::2] = 1.0
+    want[::2] = l.argmax(-1)[::2]
+    assert not torch.equal(sample_tokens(l, u)[::2], want[::2])  # the draw itself is another token
+    for name in ("temperature", "top_p", "min_p"):
+        x = bad.clone()
+        if name == "min_p":
+            x[1::2] = 0.0
+        assert torch.equal(sample_tokens(l, u, **{name: x}), want), name
