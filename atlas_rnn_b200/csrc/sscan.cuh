@@ -393,6 +393,13 @@ __global__ void __launch_bounds__(32 * kWarps, kFwdCtas) k_sscan_fwd(const ScanA
 // chunk c. A thread takes 4 states of a channel, its loads kAhead records ahead of the serial chain: as a prologue of
 // every chunk's warps it cost 42 us of 70 at 64 chunks.
 constexpr int kCarryThr = 128, kAhead = 8;
+// 2^x h + e of a chunk that multiplies the state by 2^x. Where the states grow (dt A > 0), 2^x may overflow although its
+// product with h does not: by halves, and a state of 0 stays out of it.
+__device__ __forceinline__ float past_chunk(float x, float h, float e) {
+  if (x < 127.f) return fmaf(ex2(x), h, e);
+  const float half = ex2(0.5f * x);
+  return h == 0.f ? e : fmaf(h * half, half, e);
+}
 template <int NP, bool BACK>
 __global__ void __launch_bounds__(kCarryThr) k_sscan_carry(const ScanArgs a) {
   const int64_t i = (int64_t)blockIdx.x * kCarryThr + threadIdx.x, row = i / (NP / 4);  // b * Dm + d
@@ -422,10 +429,10 @@ __global__ void __launch_bounds__(kCarryThr) k_sscan_carry(const ScanArgs a) {
     for (int k = 0; k < kAhead; ++k) {
       if (c0 + k >= a.nchunk) break;
       *reinterpret_cast<float4*>(a.part_h + (first + (c0 + k) * step) * NP + n4) = make_float4(h[0], h[1], h[2], h[3]);
-      h[0] = fmaf(ex2(A[0] * dt[k]), h[0], e[k].x);
-      h[1] = fmaf(ex2(A[1] * dt[k]), h[1], e[k].y);
-      h[2] = fmaf(ex2(A[2] * dt[k]), h[2], e[k].z);
-      h[3] = fmaf(ex2(A[3] * dt[k]), h[3], e[k].w);
+      h[0] = past_chunk(A[0] * dt[k], h[0], e[k].x);
+      h[1] = past_chunk(A[1] * dt[k], h[1], e[k].y);
+      h[2] = past_chunk(A[2] * dt[k], h[2], e[k].z);
+      h[3] = past_chunk(A[3] * dt[k], h[3], e[k].w);
     }
   }
 }

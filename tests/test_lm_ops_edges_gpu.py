@@ -56,3 +56,71 @@ def test_settings_per_row_that_are_nan_give_the_first_token(native_lib, rows, V)
         if name == "min_p":
             x[1::2] = 0.0
         assert torch.equal(sample_tokens(l, u, **{name: x}), want), name
+
+
+def growth(dt, A, n, T, live, dtype=torch.float64, h0=None):
+    """One channel group of states that grow: delta dt [T], A > 0, inputs u only at the steps `live`."""
+    g = torch.Generator().manual_seed(3)
+    pos = lambda *s: 0.5 + torch.rand(*s, generator=g, dtype=dtype)
+    u = torch.zeros(1, T, 5, dtype=dtype)
+    u[:, live] = pos(1, len(live), 5)
+    x = dict(u=u, delta=dt.to(dtype)[None, :, None].expand(1, T, 5).contiguous(), A=torch.full((5, n), A, dtype=dtype),
+             B=pos(1, T, n), C=pos(1, T, n), initial_state=h0)
+    return {k: None if v is None else v.float().double() for k, v in x.items()}
+
+
+def steps(x):
+    """The recurrence in float64, one step after another."""
+    h = torch.zeros(1, 5, x["A"].shape[1], dtype=torch.float64) if x["initial_state"] is None else x["initial_state"]
+    out = []
+    for t in range(x["u"].shape[1]):
+        dt = x["delta"][:, t, :, None]
+        h = torch.exp(dt * x["A"]) * h + dt * x["u"][:, t, :, None] * x["B"][:, t, None]
+        out.append((h * x["C"][:, t, None]).sum(-1))
+    return torch.stack(out, 1), h
+
+
+def scan(x, chunk):
+    from atlas_rnn_b200 import selective_scan
+    return selective_scan(**{k: None if v is None else v.float().cuda() for k, v in x.items()}, chunk=chunk)
+
+
+@pytest.mark.parametrize("n", [3, 16])
+def test_growing_states_whose_factor_over_a_chunk_overflows(native_lib, n):
+    """e^(dt A) = e^4 a step: e^128, beyond fp32, over a chunk of 32, whose entering state is 0 (inputs in the last 8 steps
+    alone). All terms are positive. A step's factor is off by at most 2^-22 (the hardware's exp2) + 4 2^-23 (the roundings of
+    its argument) < 2^-20, over 7 steps, and the sums by n 2^-24: 2^-16 covers both."""
+    x = growth(torch.full((96,), 4.0), 1.0, n, 96, list(range(88, 96)))
+    out, hT = steps(x)
+    for chunk in (0, 32, 64, 96):
+        got = scan(x, chunk)
+        torch.testing.assert_close(got[0].double().cpu(), out, rtol=2.0 ** -16, atol=0)
+        torch.testing.assert_close(got[1].double().cpu(), hT, rtol=2.0 ** -16, atol=0)
+
+
+def test_growing_gradients_whose_factor_over_a_chunk_overflows(native_lib):
+    """The same backwards: outputs are used in the first 8 steps, and no gradient enters from behind."""
+    x = growth(torch.full((96,), 4.0), 1.0, 3, 96, [])
+    x["u"][:, 88:] = 1.0
+    leaf = {k: None if v is None else v.clone().requires_grad_() for k, v in x.items()}
+    steps(leaf)[0][:, :8].sum().backward()
+    from atlas_rnn_b200 import selective_scan
+    for chunk in (0, 32, 64, 96):
+        mine = {k: None if v is None else v.float().cuda().requires_grad_() for k, v in x.items()}
+        selective_scan(**mine, chunk=chunk)[0][:, :8].sum().backward()
+        for k, v in leaf.items():
+            if v is not None:
+                torch.testing.assert_close(mine[k].grad.double().cpu(), v.grad, rtol=2.0 ** -16, atol=0, msg=lambda m: f"{k}: {m}")
+
+
+def test_a_tiny_state_that_grows_by_more_than_the_largest_number(native_lib):
+    """A chunk's factor of e^92.8 = 2^133.9 overflows; times the state of 1.2e-37 it does not. dt A is added over 32 steps
+    and multiplied by log2(e), 6 roundings of 2^-24 of 133.9 ln 2 = 93 at most: 4e-5; step by step as much. 2^-13."""
+    dt = torch.full((64,), 2.9)
+    dt[32:] = 0.0
+    x = growth(dt, 1.0, 3, 64, [], h0=torch.full((1, 5, 3), 1.2e-37, dtype=torch.float64))
+    out, hT = steps(x)
+    for chunk in (32, 64):
+        got = scan(x, chunk)
+        torch.testing.assert_close(got[0][:, 32:].double().cpu(), out[:, 32:], rtol=2.0 ** -13, atol=0)
+        torch.testing.assert_close(got[1].double().cpu(), hT, rtol=2.0 ** -13, atol=0)
