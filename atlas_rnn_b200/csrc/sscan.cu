@@ -172,7 +172,8 @@ int step_t(const AtlasSelScan* a, ScanArgs s, cudaStream_t st) {
 
 template <class IO, int NP, bool Z>
 int bwd_t(const AtlasSelScan* a, ScanArgs s, const BwdLayout& L, cudaStream_t st) {
-  const int64_t rows = a->B * a->T;
+  const int64_t rows = a->B * a->T, blocks = (rows * 2 * NP / 4 + 255) / 256;
+  if (a->dB && blocks > 0x7fffffff / a->G) return ATLAS_ERR_UNSUPPORTED;  // before the first launch
   const int tiles = tiles_of(a, NP, kMcBwd<NP>);
   alignment(a, s, 16 / (int)sizeof(IO));
   if (s.nchunk > 1) {
@@ -184,10 +185,8 @@ int bwd_t(const AtlasSelScan* a, ScanArgs s, const BwdLayout& L, cudaStream_t st
   if (const int rc = walk(KID_SSCAN_BWD, k_sscan_bwd<IO, NP, Z>, a, s, tiles, s.nchunk, (int)sizeof(BwdSmem<IO, NP, Z>), st))
     return rc;
   if (a->dB) {
-    const int64_t blocks = (rows * 2 * NP / 4 + 255) / 256;
-    if (blocks > 0x7fffffff || a->G > 65535) return ATLAS_ERR_UNSUPPORTED;
-    LAUNCH_T(KID_SSCAN_DBC, (k_sscan_dbc<IO, NP>), dim3((unsigned)blocks, a->G), 256, 0, st, s.dbc, (IO*)a->dB,
-             (IO*)a->dC, rows, a->N, a->G, tiles_of(a, NP, kMcBwd<NP>));
+    LAUNCH_T(KID_SSCAN_DBC, (k_sscan_dbc<IO, NP>), dim3((unsigned)(blocks * a->G)), 256, 0, st, s.dbc, (IO*)a->dB,
+             (IO*)a->dC, rows, a->N, a->G, tiles_of(a, NP, kMcBwd<NP>), (unsigned)blocks);
   }
   const int64_t n = (int64_t)a->D * NP + 2 * (int64_t)a->D;
   LAUNCH_T(KID_SSCAN_DA, k_sscan_dA, dim3((unsigned)((n + 255) / 256)), 256, 0, st, s.part_dA, s.part_dD, a->dA, a->dD,

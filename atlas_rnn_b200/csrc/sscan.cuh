@@ -924,13 +924,13 @@ __global__ void __launch_bounds__(32 * kWarps, kBwdCtas) k_sscan_bwd(const ScanA
 }
 
 // d B, d C: the sum of the channel tiles' records, in tile order. One thread per 4 states; rows past the
-// length hold zeros.
+// length hold zeros. grid: `blocks` for each group.
 template <class IO, int NP>
 __global__ void __launch_bounds__(256) k_sscan_dbc(const float* dbc, IO* dB, IO* dC, int64_t rows, int N, int G,
-                                                   int tiles) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;  // over [rows, 2, NP] of group blockIdx.y
+                                                   int tiles, unsigned blocks) {
+  const int g = blockIdx.x / blocks;
+  const int64_t i = ((int64_t)(blockIdx.x - g * blocks) * 256 + threadIdx.x) * 4;  // over the group's [rows, 2, NP]
   if (i >= rows * 2 * NP) return;
-  const int g = blockIdx.y;
   const float* p = dbc + (int64_t)g * tiles * rows * 2 * NP + i;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8

@@ -124,3 +124,27 @@ def test_a_tiny_state_that_grows_by_more_than_the_largest_number(native_lib):
         got = scan(x, chunk)
         torch.testing.assert_close(got[0][:, 32:].double().cpu(), out[:, 32:], rtol=2.0 ** -13, atol=0)
         torch.testing.assert_close(got[1].double().cpu(), hT, rtol=2.0 ** -13, atol=0)
+
+
+def test_more_groups_than_a_grid_is_high(native_lib):
+    """70000 groups of one channel: gradients of B and C against float64. Sums of 1 channel over at most 3 steps: products
+    of up to 6 factors each rounded, exponentials off by 2^-20; 2^-17 of the largest term covers them."""
+    from atlas_rnn_b200 import selective_scan
+    g = torch.Generator().manual_seed(0)
+    b, t, d, n = 1, 3, 70000, 2
+    rn = lambda *s: torch.randn(*s, generator=g)
+    x = dict(u=rn(b, t, d), delta=rn(b, t, d).abs(), A=-rn(d, n).abs(), B=rn(b, t, d, n), C=rn(b, t, d, n))
+    ref = {k: v.double().requires_grad_() for k, v in x.items()}
+    h, out = 0, []
+    for i in range(t):
+        dt = ref["delta"][:, i, :, None]
+        h = torch.exp(dt * ref["A"]) * h + dt * ref["u"][:, i, :, None] * ref["B"][:, i]
+        out.append((h * ref["C"][:, i]).sum(-1))
+    torch.stack(out, 1).sum().backward()
+    mine = {k: v.cuda().requires_grad_() for k, v in x.items()}
+    got = selective_scan(**mine)[0]
+    got.sum().backward()
+    torch.testing.assert_close(got.double().cpu(), torch.stack(out, 1), rtol=0, atol=2.0 ** -17 * 100)
+    for k, v in ref.items():
+        torch.testing.assert_close(mine[k].grad.double().cpu(), v.grad, rtol=0, atol=2.0 ** -17 * v.grad.abs().max().item(),
+                                   msg=lambda m: f"{k}: {m}")
