@@ -20,6 +20,8 @@ struct Plan {
   int chunk, nchunk;  // time axis
 };
 
+constexpr int kMaxChunks = 65535;  // the second dimension of a grid
+
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
 int tiles_of(const AtlasSelScan* a, int np, int mc) {  // channel tiles (CTAs) of one group
@@ -38,7 +40,9 @@ void cut(const AtlasSelScan* a, int mc, int resident, int waves, Plan& p) {
   auto steps = [&](int64_t n) { return (a->T + n - 1) / n; };
   int64_t c = std::max(steps(many), std::min<int64_t>(256, steps(fill)));
   if (waves > 1 && wave / ctas < 1) c = a->T;
-  c = a->chunk > 0 ? a->chunk : round_up(std::max<int64_t>(c, 32), kTT);
+  // a chunk asked for is lengthened where a grid could not hold as many of them
+  const int64_t least = round_up((a->T + kMaxChunks - 1) / kMaxChunks, 32);
+  c = a->chunk > 0 ? std::max<int64_t>(a->chunk, least) : round_up(std::max<int64_t>(c, 32), kTT);
   c = std::min<int64_t>(c, round_up(a->T, kTT));
   p.chunk = (int)std::min<int64_t>(c, (int64_t)1 << 30);
   p.nchunk = (int)((a->T + p.chunk - 1) / p.chunk);
@@ -123,7 +127,7 @@ void alignment(const AtlasSelScan* a, ScanArgs& s, int bc) {
 template <class K>
 int walk(int kid, K kernel, const AtlasSelScan* a, const ScanArgs& s, int tiles, int chunks, int bytes, cudaStream_t st) {
   const int64_t gx = a->B * a->G * tiles;
-  if (gx > 0x7fffffff || chunks > 65535) return ATLAS_ERR_UNSUPPORTED;
+  if (gx > 0x7fffffff || chunks > kMaxChunks) return ATLAS_ERR_UNSUPPORTED;
   if (bytes > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
     return ATLAS_ERR_LAUNCH;
   LAUNCH_T(kid, kernel, dim3((unsigned)gx, chunks), 32 * kWarps, bytes, st, s);

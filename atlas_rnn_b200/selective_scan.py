@@ -253,7 +253,7 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D:
     floating input. The sums over steps, states and channels are in float32 and in a fixed order, so the same call gives the
     same bits. A training call keeps the states of every 8th step for its backward (d n / 8 floats a step).
     One step without gradients runs one small kernel. chunk: steps per piece of a cut time axis (a multiple
-    of 32; 0 lets the library choose)."""
+    of 32, lengthened where t takes more than 65535 pieces; 0 lets the library choose)."""
     if _through_autograd(u, delta, A, B, C, D, z, delta_bias, initial_state):
         return SelectiveScanFn.apply(u, delta, A, B, C, D, z, delta_bias, initial_state, lengths, delta_softplus, chunk)
     return _scan_operands(u, delta, A, B, C, D, z, delta_bias, initial_state, lengths, delta_softplus,

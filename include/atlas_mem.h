@@ -423,7 +423,7 @@ typedef struct AtlasSelScan {
   int32_t D, N, G;
   int32_t softplus;
   int32_t dtype_io;
-  int32_t chunk;    /* steps per time chunk, a multiple of 32; 0: library default */
+  int32_t chunk;    /* steps per time chunk, a multiple of 32 (more where T takes over 65535 of them); 0: library default */
   const void *u, *delta, *z, *Bm, *Cm;
   int64_t u_sb, u_st, delta_sb, delta_st, z_sb, z_st, B_sb, B_st, B_sg, C_sb, C_st, C_sg;
   const float *A, *Dskip, *bias, *h0;

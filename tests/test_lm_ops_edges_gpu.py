@@ -148,3 +148,24 @@ def test_more_groups_than_a_grid_is_high(native_lib):
     for k, v in ref.items():
         torch.testing.assert_close(mine[k].grad.double().cpu(), v.grad, rtol=0, atol=2.0 ** -17 * v.grad.abs().max().item(),
                                    msg=lambda m: f"{k}: {m}")
+
+
+def test_short_chunks_of_a_long_row(native_lib):
+    """More chunks than a grid is high (65535). dt A = -1 a step: what a state was 64 steps ago is left by e^-64, so the last
+    steps are those of a scan of the last 256 alone, bit for bit up to the cut's roundings (2^-20 a step, 2^-17 in all)."""
+    from atlas_rnn_b200 import selective_scan
+    g = torch.Generator(device="cuda").manual_seed(0)
+    T = 65536 * 32 + 5
+    pos = lambda *s: 0.5 + torch.rand(*s, device="cuda", generator=g)
+    x = dict(u=pos(1, T, 2), delta=torch.ones(1, T, 2, device="cuda"), B=pos(1, T, 1), C=pos(1, T, 1))
+    A = -torch.ones(2, 1, device="cuda")
+    tail = {k: v[:, -256:].clone().requires_grad_() for k, v in x.items()}
+    want, hT = selective_scan(A=A, **tail, chunk=256)
+    (want[:, 64:].sum() + hT.sum()).backward()
+    x = {k: v.requires_grad_() for k, v in x.items()}
+    got, last = selective_scan(A=A, **x, chunk=32)
+    (got[:, -192:].sum() + last.sum()).backward()
+    torch.testing.assert_close(got[:, -192:], want[:, 64:], rtol=2.0 ** -17, atol=0)
+    torch.testing.assert_close(last, hT, rtol=2.0 ** -17, atol=0)
+    for k, v in tail.items():
+        torch.testing.assert_close(x[k].grad[:, -192:], v.grad[:, 64:], rtol=2.0 ** -17, atol=2.0 ** -17 * v.grad.abs().max().item())
