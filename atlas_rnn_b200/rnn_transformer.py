@@ -159,7 +159,7 @@ class RNNMemoryTransformer(Module):
                 logits, states, _ = self(x, mem_states=states, return_cache=True)
             else:
                 logits = self(full)
-            if top_k > 0 or top_p < 1.0:
+            if top_k != 0 or top_p != 1.0:  # what is out of range (a NaN too) is refused there
                 last = logits[:, -1:]
                 last = last if last.dtype == torch.bfloat16 else last.float()
                 nxt = sample_tokens(last, torch.rand(last.shape, device=last.device), temperature=temperature,

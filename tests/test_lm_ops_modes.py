@@ -55,3 +55,13 @@ def test_tensors_of_the_host_are_refused(call):
 def test_other_sizes_and_types_are_refused(call, change, error):
     with pytest.raises(error, match="atlas_rnn_b200"):
         call(**change)
+
+
+@pytest.mark.parametrize("settings", [dict(top_k=-1), dict(top_p=float("nan")), dict(top_p=1.5), dict(top_p=-0.5),
+                                      dict(top_k=5, min_p=2.0), dict(top_k=0.5)])
+def test_generate_refuses_settings_out_of_range(settings, monkeypatch):
+    import atlas_rnn_b200 as A
+    m = A.RNNMemoryTransformer(num_tokens=8, dim=8, depth=1, heads=1, dim_head=8)
+    monkeypatch.setattr(m, "forward", lambda x, **_: (Z(*x.shape, 8), None, None))
+    with pytest.raises((ValueError, TypeError), match="top_k|top_p|min_p|integer"):
+        m.generate(Z(1, 3, dtype=torch.int64), max_length=4, **settings)
