@@ -169,3 +169,31 @@ def test_short_chunks_of_a_long_row(native_lib):
     torch.testing.assert_close(last, hT, rtol=2.0 ** -17, atol=0)
     for k, v in tail.items():
         torch.testing.assert_close(x[k].grad[:, -192:], v.grad[:, 64:], rtol=2.0 ** -17, atol=2.0 ** -17 * v.grad.abs().max().item())
+
+
+def test_generate_passes_every_filter_on(native_lib):
+    """At temperature 1, each filter alone leaves the most likely token; and with all of them the tokens are those of a loop
+    over sample_tokens with the same uniforms."""
+    import atlas_rnn_b200 as A
+    torch.manual_seed(0)
+    m = A.RNNMemoryTransformer(num_tokens=64, dim=32, depth=1, heads=1, dim_head=32, omega_window=2).cuda()
+    prompt = torch.randint(0, 64, (3, 5), device="cuda")
+    greedy = m.generate(prompt, max_length=20, temperature=0.0)
+    free = dict(max_length=20, temperature=1.0, min_p=0.0)
+    assert not torch.equal(m.generate(prompt, **free, top_k=63), greedy)
+    assert torch.equal(m.generate(prompt, **free, top_p=1e-9), greedy)
+    assert torch.equal(m.generate(prompt, **free, top_k=1), greedy)
+    assert torch.equal(m.generate(prompt, max_length=20, temperature=1.0, min_p=1.0, top_k=63), greedy)
+
+    cfg = dict(temperature=0.7, top_k=30, top_p=0.8, min_p=0.01)
+    torch.manual_seed(1)
+    got = m.generate(prompt, max_length=20, **cfg)
+    torch.manual_seed(1)
+    full, x, states = prompt, prompt, None
+    with torch.no_grad():
+        for _ in range(15):
+            logits, states, _ = m(x, mem_states=states, return_cache=True)
+            last = logits[:, -1:].float()
+            x = A.sample_tokens(last, torch.rand(last.shape, device="cuda"), **cfg)
+            full = torch.cat([full, x], dim=-1)
+    assert torch.equal(got, full) and not torch.equal(got, greedy)
