@@ -143,3 +143,51 @@ def test_traced_distillation(native_lib):
     same(f, m, x.t().contiguous().t(), v.double(), i.int())
     with pytest.raises(Exception, match="teacher_values must have shape"):
         m(x, v[:3], i)
+
+
+@pytest.mark.parametrize("t", [1, 40])
+def test_function_transforms_are_refused(native_lib, t):
+    """torch.func's wrappers have no storage that a kernel could read."""
+    from atlas_rnn_b200 import causal_conv1d, distill_loss, sample_tokens, selective_scan
+    x = scan_inputs(2, t, 6, 4, seed=1)
+    w, v = rand(6, 4, seed=2), rand(t, 3, seed=3)
+    i = torch.zeros(t, 3, dtype=torch.int64, device="cuda")
+    calls = [lambda u: selective_scan(**{**x, "u": u})[0], lambda u: causal_conv1d(u, w)[0],
+             lambda u: distill_loss(u, v.expand(2, t, 3), i.expand(2, t, 3))]
+    for f in calls:
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (x["u"],), (torch.ones_like(x["u"]),))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda u: f(u).sum())(x["u"])
+    for f in calls[:2] + [lambda u: sample_tokens(u, u.sigmoid())]:
+        with pytest.raises(RuntimeError):
+            torch.vmap(f)(x["u"][None].expand(3, *x["u"].shape).contiguous())
+
+
+def test_recomputed_and_offloaded_training_steps(native_lib):
+    """Gradients under activation checkpointing and with the kept tensors moved to the host are the plain step's bits."""
+    from torch.utils.checkpoint import checkpoint
+    from atlas_rnn_b200 import causal_conv1d, selective_scan
+    x, w = scan_inputs(2, 70, 6, 4, seed=1), rand(6, 4, seed=2)
+    names = list(x)
+
+    def layer(*a):
+        s = dict(zip(names, a[1:]))
+        s["u"] = causal_conv1d(s["u"], a[0], activation="silu")[0]
+        out, hT = selective_scan(**s, delta_softplus=True)
+        return out.square().sum() + hT.sum()
+
+    def grads(run):
+        leaves = [w.clone().requires_grad_()] + [v.clone().requires_grad_() for v in x.values()]
+        run(leaves).backward()
+        return [v.grad for v in leaves]
+
+    want = grads(lambda a: layer(*a))
+    offloaded = grads(lambda a: offload(layer, a))
+    for got in (grads(lambda a: checkpoint(layer, *a, use_reentrant=False)), offloaded):
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def offload(f, args):
+    with torch.autograd.graph.save_on_cpu():
+        return f(*args)
