@@ -119,9 +119,8 @@ def _io(t: Tensor | None, dtype) -> Tensor | None:
 
 
 def _has_tangent(*tensors) -> bool:
-    """Whether a tensor carries a forward-mode tangent (a dual tensor's requires_grad is False)."""
-    return forward_ad._current_level >= 0 and any(
-        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    """Whether a tensor carries a forward-mode tangent (a dual tensor's requires_grad is False). Inside a dual level."""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def decode_supported(spec: Spec, d_k: int, d_phi: int, d_v: int) -> bool:
@@ -343,8 +342,8 @@ def memory_recurrence(k: Tensor, q: Tensor, v: Tensor, lr: Tensor, decay: Tensor
     args = (_io(k, io), _io(q, io), _io(v, io), _io(lr, io), _io(decay, io), _io(beta, io), _io(gate, io),
             f32(S_ref), f32(S0), Z0c, buf, projc)
     inputs = (k, q, v, lr, decay, beta, gate, S_ref, S0, Z0, omega_buffer)
-    needs_grad = torch.jit.is_tracing() or _has_tangent(*inputs) or torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in inputs)
+    needs_grad = torch._C._is_tracing() or forward_ad._current_level >= 0 and _has_tangent(*inputs) \
+        or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
     if (heads_padded_from is None and k.shape[1] == 1 and not needs_grad
             and decode_supported(spec, k.shape[-1], S_ref.shape[-1], v.shape[-1])):
         y, S_end, Z_end, buf_out = decode_step(spec, *args)

@@ -16,6 +16,7 @@ import struct
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -87,8 +88,11 @@ def _through_autograd(*tensors) -> bool:
     function refuses (a call past it would drop the tangent); and for a trace, which would have no more of a call past it than
     the allocation of the outputs. Else the call itself saves the detour's time. The function holds the checks and layouts
     too: a traced call does them on the inputs that it is run with."""
-    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) \
-        or torch.jit.is_tracing() or _has_tangent(*tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return torch._C._is_tracing() or (forward_ad._current_level >= 0 and _has_tangent(*tensors))
 
 
 def _run(what: str, fn, device, *args):
