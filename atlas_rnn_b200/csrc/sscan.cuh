@@ -34,8 +34,8 @@ namespace ss {
 
 // Channels per lane, forward and backward. Forward 4: fewer shared-memory loads and instructions a state (measured at
 // B 4, T 8192, D 1536, N 16, bf16: 350 us; 2 with as many or more warps 5-15% more). Backward 2: the states of
-// kTT steps stay in 168 registers (986 us; 4 needs 255 registers: 4-15% more). Wide states take 4: 2 would leave a
-// warp less than 16 bytes of a row.
+// kTT steps stay in 168 registers (986 us; 4 needs 255 registers: 4-15% more), but for spills of 8-144 bytes (N over 32:
+// 640-896). Wide states take 4: 2 would leave a warp less than 16 bytes of a row.
 constexpr int kMcFwd = 4;
 template <int NP>
 constexpr int kMcBwd = NP < 64 ? 2 : 4;

@@ -97,7 +97,8 @@ def distill_loss(logits: Tensor, teacher_values: Tensor, teacher_indices: Tensor
         loss = temperature^2 sum_k p_k (log p_k - log q[index_k])
 
     and 0 (without a gradient) for a row that has no entries. reduction 'none' returns float32 [...]; 'sum' the sum; 'mean'
-    the mean over the rows with entries (0 when there are none). Gradients go to the logits alone."""
+    the mean over the rows with entries (0 when there are none). Gradients go to the logits alone. Sums and logarithms
+    are float32: a row's loss is exact to about temperature^2 log2(V) 2^-22, which counts where high temperatures make p and q alike."""
     if reduction not in ("none", "mean", "sum"):
         raise ValueError(f"atlas_rnn_b200.distill_loss: reduction must be 'none', 'mean' or 'sum', not {reduction!r}")
     loss, valid = DistillLossFn.apply(logits, teacher_values.detach(), teacher_indices, float(temperature))

@@ -92,7 +92,8 @@ def sample_tokens(logits: Tensor, noise: Tensor, *, temperature=1.0, top_k=0, to
     the logits beforehand for filters on the tempered distribution. Each setting is a number or a tensor with one value
     per row (a row with a NaN among them gets its first token). Masked tokens are -inf (NaN counts as -inf); a row with
     nothing above -inf gives 0.
-    V up to 2^24 - 16. Returns int64 [...], the same whatever the batch: scores are compared in float64, the probabilities
-    that the filters add up are exact to 2^-23 each."""
-    call = SampleTokensFn.apply if torch.jit.is_tracing() else _sample
+    V up to 2^24 - 16. Returns int64 [...], the same whatever the batch: scores are compared in float64; the probabilities
+    that the filters add up are float32 exponentials, each exact to 2^-21 of the largest one (a token d below the maximum to
+    (d + 1) 2^-22 of its own and 2^-40 of the largest), and are added exactly."""
+    call = SampleTokensFn.apply if torch._C._is_tracing() else _sample
     return call(logits, noise, temperature, top_k, top_p, min_p)

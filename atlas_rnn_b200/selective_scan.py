@@ -255,7 +255,8 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D:
     int64): steps at or past a row's length are not read, leave its state alone and give 0.
     Returns (out [b, t, d] in u's type, final state [b, d, n] float32); both carry gradients to every
     floating input. The sums over steps, states and channels are in float32 and in a fixed order, so the same call gives the
-    same bits. A training call keeps the states of every 8th step for its backward (d n / 8 floats a step).
+    same bits. A training call keeps the states of every 8th step for its backward (d / 8 floats a step for each
+    state, n counted as 8, 16, 32 or 64).
     One step without gradients runs one small kernel. chunk: steps per piece of a cut time axis (a multiple
     of 32, lengthened where t takes more than 65535 pieces; 0 lets the library choose)."""
     if _through_autograd(u, delta, A, B, C, D, z, delta_bias, initial_state):
