@@ -44,10 +44,23 @@ def _stream(dev) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
+def _on_one_device(*tensors):
+    """Kernels read the operands' addresses: all of them on the first one's CUDA device. (memory_recurrence's own check of k
+    is no part of a traced call.)"""
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise RuntimeError("atlas_rnn_b200.memory_recurrence: tensors must be on a CUDA device "
+                           "(the library has no CPU path)")
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"atlas_rnn_b200.memory_recurrence: operands on {dev} and {t.device}")
+
+
 class MemoryRecurrenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, spec: Spec, k, q, v, lr, decay, beta, gate, S_ref, S0, Z0, buf, proj):
         ctx.set_materialize_grads(False)  # unused outputs arrive as None, not zero tensors
+        _on_one_device(k, q, v, lr, decay, beta, gate, S_ref, S0, Z0, buf, proj)
         dev = k.device
         N, T, _ = k.shape
         d_phi = S_ref.shape[-1]
@@ -132,6 +145,7 @@ def decode_step(spec: Spec, k, q, v, lr, decay, beta, gate, S_ref, S0, Z0, buf, 
     """One token (T = 1) through atlas_mem_decode_step: inference only, no autograd
     graph, no workspaces. Operands as for MemoryRecurrenceFn (io dtype for k..gate,
     fp32 states)."""
+    _on_one_device(k, q, v, lr, decay, beta, gate, S_ref, S0, Z0, buf, proj)
     dev = k.device
     N, T, _ = k.shape
     d_phi, d_v = S_ref.shape[-1], v.shape[-1]
